@@ -1,0 +1,500 @@
+// The k best continuations of a request's beams (b200_beam_select): log softmax over every beam's logits, the beam's score added, and the k
+// best of beams x vocabulary in the order of (score in 64 bits, beam, token).
+//
+//   score(b, w) = scores[b] + ((x_w - m) - log sum_v exp(x_v - m)),   m = max_v x_v        (m = +inf: x_w - m is 0 where x_w = m, -inf elsewhere)
+//
+// Bound by reading the logits once.  Two launches:
+//   * beam_rows_kernel: a CTA holds a chunk of a row in registers (256 threads x EPT values), so that maximum, sum of exponentials and the chunk's k best come of
+//     one read.  The k best: the k-th largest of the threads' own maxima is a bound that at least k values reach and few more do; a bisection
+//     over counts (one barrier each) comes near enough to it, the values above are listed and ordered by counting the better ones of each.
+//     Where too many reach the bound (equal values), the bisection goes on over all values, then over the indexes of the equal ones.
+//   * beam_merge_kernel: a CTA per request joins the chunks' sums in 64 bits and selects among beams x chunks x k candidates the same way, the scores
+//     in 64 bits: two candidates of different beams are told apart unless their scores agree to about 1e-8.
+// Sums: F32 over a thread's values, 64 bits from there (1e-7 of the sum, so 1e-7 of a score).  The same row gives the same bits wherever it lies:
+// which thread sums which value depends on the vocabulary alone, also where rows do not begin at 16-byte boundaries (their values are then shifted into place).
+#include <cuda_bf16.h>
+
+#include "paged.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int BS_NT = 256, BS_MAX_K = 128, BS_MAX_BEAM = 64;
+constexpr int BS_LIST = 512;            // candidates that are ordered by counting
+constexpr int BS_MERGE_NT = 512, BS_CACHE = 4096;   // 32 KB of scores
+
+struct Cand {                            // of a chunk, in descending order
+    float value;
+    int token;
+};
+struct SelectArgs {
+    const uint8_t *logits;
+    const float *scores;
+    const uint8_t *done;
+    int64_t ld, n_vocab;
+    int n_beam, k, chunks, end_token;
+    Cand *cand;                          // [row][chunk][k]
+    int *count;                          // [row][chunk]
+    float *top;                          // [row][chunk]
+    double *sum;                         // [row][chunk]
+    float *out_scores;
+    int32_t *out_tokens, *out_parents;
+};
+
+// an integer in the order of the float (no NaN; -0 is +0)
+__device__ __forceinline__ uint32_t order32(float x) {
+    const uint32_t b = __float_as_uint(x + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order64(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
+    return b >> 63 ? ~b : b | (1ull << 63);
+}
+constexpr uint32_t ORDER32_NONE = 0x007fffffu;               // of -inf
+constexpr uint64_t ORDER64_NONE = 0x000fffffffffffffull;
+
+__device__ __forceinline__ int block_count(bool p) { return __syncthreads_count(p); }
+__device__ __forceinline__ int block_total(int v, int *part) {   // sum over the block; part: one int per warp
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    int t = 0;
+    for (int i = 0; i < (int)(blockDim.x >> 5); i++) t += part[i];
+    return t;
+}
+
+// the 16 bytes at p, which need not be aligned; [lo, hi): the bytes that may be read in whole words around them
+template <typename T>
+__device__ __forceinline__ void load16(const uint8_t *p, const uint8_t *row_end, const uint8_t *lo, const uint8_t *hi, uint32_t (&w)[4]) {
+    constexpr int N = 16 / (int)sizeof(T);
+    const int shift = (int)((uintptr_t)p & 15);
+    if (shift == 0 && p + 16 <= row_end) {
+        const uint4 v = ld_stream16(p);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        return;
+    }
+    const uint8_t *const a = p - shift;
+    if (p + 16 <= row_end && a >= lo && a + 32 <= hi) {
+        const uint4 v0 = *(const uint4 *)a, v1 = *(const uint4 *)(a + 16);
+        const uint32_t in[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+        const int words = shift >> 2, bits = (shift & 3) * 8;   // the same for a whole row
+        uint32_t s[5];
+#pragma unroll
+        for (int i = 0; i < 5; i++) s[i] = words == 0 ? in[i] : words == 1 ? in[i + 1] : words == 2 ? in[i + 2] : (i + 3 < 8 ? in[i + 3] : 0u);
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(s[i], s[i + 1], bits);
+        return;
+    }
+    // value by value at the tensor's ends
+    const T none = (T)(-INFINITY);
+    __align__(16) T e[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) e[i] = p + (i + 1) * (int)sizeof(T) <= row_end ? ((const T *)p)[i] : none;
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = ((const uint32_t *)e)[i];
+}
+
+template <typename T>
+struct Unpack;
+template <>
+struct Unpack<float> {
+    static constexpr int N = 4;
+    __device__ static void get(const uint32_t (&w)[4], float *v) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(w[i]);
+    }
+};
+template <typename T>
+struct Unpack {
+    static constexpr int N = 8;
+    __device__ static void get(const uint32_t (&w)[4], float *v) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = paged_two<T>(w[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+};
+
+// EPT values a thread, a vector of 16 bytes at a time: value N j + i of vector v of thread t is element chunk * BS_NT * EPT + (v * BS_NT + t) * N + i
+template <typename T, int EPT>
+__global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
+    constexpr int N = Unpack<T>::N, VECS = EPT / N;
+    pdl_trigger();
+    __shared__ float warp_top[BS_NT / 32];
+    __shared__ double warp_sum[BS_NT / 32];
+    __shared__ uint64_t list[BS_LIST];       // order of the value, then the complement of the token: larger is better
+    __shared__ int n_list, part[BS_NT / 32];
+    const int tid = threadIdx.x, chunk = blockIdx.x;
+    const int64_t row = blockIdx.y;
+    const int64_t slot = row * a.chunks + chunk;
+    pdl_wait();
+    if (a.done && a.done[row]) return;       // the merge does not ask for this beam
+    const uint8_t *const base = a.logits + row * a.ld * (int64_t)sizeof(T), *const row_end = base + a.n_vocab * (int64_t)sizeof(T);
+    const int first = chunk * BS_NT * EPT;   // the vocabulary is below 2^31
+    float x[EPT];
+#pragma unroll
+    for (int v = 0; v < VECS; v++) {
+        const int64_t e = (int64_t)first + (int64_t)(v * BS_NT + tid) * N;
+        if (e < a.n_vocab) {
+            uint32_t w[4];
+            load16<T>(base + e * (int64_t)sizeof(T), row_end, base, row_end, w);
+            Unpack<T>::get(w, x + v * N);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) x[v * N + i] = -INFINITY;
+        }
+    }
+    float mine = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+        if (x[i] != x[i]) x[i] = -INFINITY;
+        mine = fmaxf(mine, x[i]);
+    }
+    float m = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((tid & 31) == 0) warp_top[tid >> 5] = m;
+    if (tid == 0) n_list = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BS_NT / 32; i++) m = fmaxf(m, warp_top[i]);
+    // sum of exponentials
+    float s = 0.0f;
+    if (m > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < EPT; i++) s += x[i] == m ? 1.0f : exp2f((x[i] - m) * 1.4426950408889634f);
+    }
+    double ds = (double)s;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
+    if ((tid & 31) == 0) warp_sum[tid >> 5] = ds;
+    // a bound that k values of the chunk reach: bisected until few more threads than that have one (then the list has room for what
+    // independent values put above it: at 192 of 256 threads about 355)
+    uint32_t lo = ORDER32_NONE + 1, hi = order32(m);   // k values reach lo, or lo lets every finite value pass
+    const uint32_t best = order32(mine);
+    const int enough = 2 * a.k < 192 ? 2 * a.k : 192;
+    uint32_t top = hi;
+    if (block_count(best >= lo) > enough) {
+        while (lo < top) {
+            const uint32_t at = lo + (top - lo + 1) / 2;
+            const int c = block_count(best >= at);
+            if (c >= a.k) {
+                lo = at;
+                if (c <= enough) break;
+            } else {
+                top = at - 1;
+            }
+        }
+    }
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < EPT; i++) n += order32(x[i]) >= lo;
+    n = block_total(n, part);
+    int last = 0x7fffffff;       // of the values that equal the bound only those up to this token
+    if (n > BS_LIST) {           // the k-th largest value itself
+        top = hi;
+        while (lo < top) {
+            const uint32_t at = lo + (top - lo + 1) / 2;
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < EPT; i++) c += order32(x[i]) >= at;
+            if (block_total(c, part) >= a.k) lo = at;
+            else top = at - 1;
+        }
+        int above = 0;
+#pragma unroll
+        for (int i = 0; i < EPT; i++) above += order32(x[i]) > lo;
+        const int want = a.k - block_total(above, part);
+        int l = first, h = (int)(a.n_vocab - 1 < (int64_t)first + BS_NT * EPT - 1 ? a.n_vocab - 1 : (int64_t)first + BS_NT * EPT - 1);
+        while (l < h) {
+            const int at = l + (h - l) / 2;
+            int c = 0;
+#pragma unroll
+            for (int i = 0; i < EPT; i++) c += order32(x[i]) == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= at;
+            if (block_total(c, part) >= want) h = at;
+            else l = at + 1;
+        }
+        last = l;
+    }
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+        const uint32_t o = order32(x[i]);
+        if (o > lo || (o == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= last)) {
+            const int at = atomicAdd(&n_list, 1);
+            if (at < BS_LIST) list[at] = (uint64_t)o << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
+        }
+    }
+    __syncthreads();
+    n = n_list < BS_LIST ? n_list : BS_LIST;
+    Cand *const out = a.cand + slot * a.k;
+    for (int i = tid; i < n; i += BS_NT) {
+        const uint64_t me = list[i];
+        int better = 0;
+        for (int j = 0; j < n; j++) better += list[j] > me;
+        if (better < a.k) {
+            const uint32_t o = (uint32_t)(me >> 32);
+            out[better].value = __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+            out[better].token = (int)~(uint32_t)me;
+        }
+    }
+    if (tid == 0) {
+        a.count[slot] = n < a.k ? n : a.k;
+        a.top[slot] = m;
+        double t = 0.0;
+#pragma unroll
+        for (int i = 0; i < BS_NT / 32; i++) t += warp_sum[i];
+        a.sum[slot] = t;
+    }
+}
+
+__global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArgs a, int n_cached) {
+    pdl_trigger();
+    extern __shared__ uint64_t cached[];     // scores of the first n_cached candidates
+    __shared__ double offset[BS_MAX_BEAM];   // score of a beam less the logarithm of its sum
+    __shared__ float top_s[BS_MAX_BEAM];
+    __shared__ uint64_t key[BS_LIST];
+    __shared__ int64_t where[BS_LIST];       // beam * vocabulary + token
+    __shared__ int n_list, part[BS_MERGE_NT / 32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t r = blockIdx.x, row0 = r * a.n_beam;
+    if (tid == 0) n_list = 0;
+    pdl_wait();
+    for (int b = warp; b < a.n_beam; b += BS_MERGE_NT / 32) {
+        const int64_t row = row0 + b;
+        const float score = a.scores[row];
+        const bool off = !(score > -INFINITY);   // -inf or NaN
+        if (a.done && a.done[row]) {
+            if (lane == 0) {
+                offset[b] = off ? -INFINITY : (double)score;
+                top_s[b] = NAN;                  // marks an ended beam
+            }
+            continue;
+        }
+        float m = -INFINITY;
+        for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, a.top[row * a.chunks + c]);
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        double s = 0.0;
+        for (int c = lane; c < a.chunks; c += 32) {
+            const float t = a.top[row * a.chunks + c];
+            if (t > -INFINITY) s += a.sum[row * a.chunks + c] * (t == m ? 1.0 : exp((double)t - (double)m));
+        }
+        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (lane == 0) {
+            offset[b] = off || m == -INFINITY ? -INFINITY : (double)score - log(s);
+            top_s[b] = m;
+        }
+    }
+    __syncthreads();
+    // candidate i of the request: beam, chunk, place in the chunk's list
+    const int per_beam = a.chunks * a.k, total = a.n_beam * per_beam;
+    auto order = [&](int i, int64_t *at) -> uint64_t {
+        const int b = i / per_beam, j = i - b * per_beam, c = j / a.k, p = j - c * a.k;
+        const float m = top_s[b];
+        const double off = offset[b];
+        if (off == -INFINITY) return ORDER64_NONE;
+        if (m != m) {
+            *at = (int64_t)b * a.n_vocab + a.end_token;
+            return j == 0 ? order64(off) : ORDER64_NONE;
+        }
+        const int64_t slot = (row0 + b) * a.chunks + c;
+        if (p >= a.count[slot]) return ORDER64_NONE;
+        const Cand cd = a.cand[slot * a.k + p];
+        *at = (int64_t)b * a.n_vocab + cd.token;
+        if (cd.value == m) return order64(off);
+        return order64(off + ((double)cd.value - (double)m));
+    };
+    // bound: k candidates reach lo.  The scores stand in shared memory where there is room for them
+    uint64_t lo = ~0ull, hi = ORDER64_NONE;
+    int64_t at = 0;
+    int n = 0;
+    for (int i = tid; i < total; i += BS_MERGE_NT) {
+        const uint64_t o = order(i, &at);
+        if (i < n_cached) cached[i] = o;
+        if (o == ORDER64_NONE) continue;
+        hi = o > hi ? o : hi;
+        lo = o < lo ? o : lo;
+        n++;
+    }
+    auto again = [&](int i) -> uint64_t { return i < n_cached ? cached[i] : order(i, &at); };   // a thread's own candidates only
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t v = __shfl_xor_sync(0xffffffffu, hi, o), u = __shfl_xor_sync(0xffffffffu, lo, o);
+        hi = v > hi ? v : hi;
+        lo = u < lo ? u : lo;
+    }
+    if (lane == 0) {
+        key[warp] = hi;
+        key[BS_MERGE_NT / 32 + warp] = lo;
+    }
+    n = block_total(n, part);
+    for (int i = 0; i < BS_MERGE_NT / 32; i++) {
+        hi = key[i] > hi ? key[i] : hi;
+        lo = key[BS_MERGE_NT / 32 + i] < lo ? key[BS_MERGE_NT / 32 + i] : lo;
+    }
+    __syncthreads();
+    uint64_t up = hi;
+    int64_t last = 0x7fffffffffffffffLL;
+    const int enough = 2 * a.k > 64 ? 2 * a.k : 64;
+    while (n > enough && lo < up) {
+        const uint64_t mid = lo + (up - lo) / 2 + ((up - lo) & 1);
+        int c = 0;
+        for (int i = tid; i < total; i += BS_MERGE_NT) c += again(i) >= mid;
+        c = block_total(c, part);
+        if (c >= a.k) {
+            lo = mid;
+            n = c;
+        } else {
+            up = mid - 1;
+        }
+    }
+    if (n > BS_LIST) {   // more candidates than that have the k-th score: the first by beam and token
+        int above = 0;
+        for (int i = tid; i < total; i += BS_MERGE_NT) above += again(i) > lo;
+        const int want = a.k - block_total(above, part);
+        int64_t l = 0, h = a.n_beam * a.n_vocab - 1;
+        while (l < h) {
+            const int64_t mid = l + (h - l) / 2;
+            int c = 0;
+            for (int i = tid; i < total; i += BS_MERGE_NT) c += order(i, &at) == lo && at <= mid;
+            if (block_total(c, part) >= want) h = mid;
+            else l = mid + 1;
+        }
+        last = l;
+    }
+    for (int i = tid; i < total; i += BS_MERGE_NT) {
+        const uint64_t o = order(i, &at);
+        if (o > lo || (o == lo && at <= last)) {
+            const int e = atomicAdd(&n_list, 1);
+            if (e < BS_LIST) {
+                key[e] = o;
+                where[e] = at;
+            }
+        }
+    }
+    __syncthreads();
+    n = n_list < BS_LIST ? n_list : BS_LIST;
+    for (int i = tid; i < n; i += BS_MERGE_NT) {
+        const uint64_t me = key[i];
+        const int64_t mine = where[i];
+        int better = 0;
+        for (int j = 0; j < n; j++) better += key[j] > me || (key[j] == me && where[j] < mine);
+        if (better < a.k) {
+            const int64_t e = r * a.k + better;
+            const uint64_t bits = me >> 63 ? me & ~(1ull << 63) : ~me;
+            a.out_scores[e] = (float)__longlong_as_double((long long)bits);
+            a.out_parents[e] = (int32_t)(mine / a.n_vocab);
+            a.out_tokens[e] = (int32_t)(mine % a.n_vocab);
+        }
+    }
+    for (int i = n + tid; i < a.k; i += BS_MERGE_NT) {
+        a.out_scores[r * a.k + i] = -INFINITY;
+        a.out_tokens[r * a.k + i] = -1;
+        a.out_parents[r * a.k + i] = -1;
+    }
+}
+
+// values a thread: 32, or fewer where that would leave SMs without a chunk
+int select_ept(int64_t rows, int64_t n_vocab) {
+    const int sms = sm_count();
+    for (int ept = 32; ept > 8; ept /= 2)
+        if (rows * ((n_vocab + BS_NT * ept - 1) / (BS_NT * ept)) >= 2 * sms) return ept;
+    return 8;
+}
+
+struct SelectPlan {
+    int ept;
+    int64_t rows, chunks;
+    size_t cand, count, top, sum, bytes;     // offsets in the workspace
+};
+size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
+    B200_REQUIRE(g.logits_type == B200_TYPE_F32 || g.logits_type == B200_TYPE_F16 || g.logits_type == B200_TYPE_BF16, "beam_select: logits of type %d are not F32, F16 or BF16", g.logits_type);
+    B200_REQUIRE(g.n_request >= 0 && g.n_request <= 65535 && g.n_beam >= 1 && g.n_beam <= BS_MAX_BEAM, "beam_select: %d requests of %d beams (up to 65535 of up to %d)", g.n_request, g.n_beam, BS_MAX_BEAM);
+    B200_REQUIRE(g.k >= 1 && g.k <= BS_MAX_K, "beam_select: %d candidates (1 to %d)", g.k, BS_MAX_K);
+    B200_REQUIRE(g.n_vocab >= 1 && g.n_vocab <= (1 << 24) && g.logits_ld >= g.n_vocab, "beam_select: a vocabulary of %lld in rows %lld apart (up to 2^24)", (long long)g.n_vocab, (long long)g.logits_ld);
+    p->rows = (int64_t)g.n_request * g.n_beam;
+    p->ept = select_ept(p->rows, g.n_vocab);
+    p->chunks = (g.n_vocab + BS_NT * p->ept - 1) / (BS_NT * p->ept);
+    B200_REQUIRE(p->rows <= 65535, "beam_select: %lld rows are too many for one launch", (long long)p->rows);
+    B200_REQUIRE(p->chunks * g.k * g.n_beam < 0x7fffffffLL, "beam_select: too many candidates of a request");
+    const size_t slots = (size_t)(p->rows * p->chunks);
+    p->cand = 0;
+    p->count = p->cand + up256(slots * g.k * sizeof(Cand));
+    p->top = p->count + up256(slots * 4);
+    p->sum = p->top + up256(slots * 4);
+    p->bytes = p->sum + up256(slots * 8);
+    return B200_STATUS_SUCCESS;
+}
+
+template <typename T>
+int launch_rows(const SelectArgs &a, const SelectPlan &p, cudaStream_t s) {
+    const dim3 grid((unsigned)p.chunks, (unsigned)p.rows);
+    switch (p.ept) {
+        case 32: return launch_pdl(beam_rows_kernel<T, 32>, grid, dim3(BS_NT), 0, s, a);
+        case 16: return launch_pdl(beam_rows_kernel<T, 16>, grid, dim3(BS_NT), 0, s, a);
+        default: return launch_pdl(beam_rows_kernel<T, 8>, grid, dim3(BS_NT), 0, s, a);
+    }
+}
+
+}  // namespace
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" {
+
+size_t b200_beam_select_workspace_nbytes(const struct b200_beam_select_args *args) {
+    SelectPlan p;
+    if (args == nullptr || select_plan(*args, &p) != B200_STATUS_SUCCESS) return 0;
+    return p.bytes ? p.bytes : 256;
+}
+
+int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
+    B200_REQUIRE(args != nullptr, "beam_select: null arguments");
+    const b200_beam_select_args &g = *args;
+    SelectPlan p;
+    int rc = select_plan(g, &p);
+    if (rc != B200_STATUS_SUCCESS) return rc;
+    if (g.n_request == 0) return B200_STATUS_SUCCESS;
+    B200_REQUIRE(g.logits != nullptr && g.scores != nullptr && g.out_scores != nullptr && g.out_tokens != nullptr && g.out_parents != nullptr, "beam_select: null operand");
+    B200_REQUIRE(g.done == nullptr || (g.end_token >= 0 && g.end_token < g.n_vocab), "beam_select: end token %d is outside the vocabulary", g.end_token);
+    const int size = g.logits_type == B200_TYPE_F32 ? 4 : 2;
+    B200_REQUIRE((uintptr_t)g.logits % size == 0, "beam_select: logits must be aligned to their type");
+    B200_REQUIRE(g.workspace != nullptr && (uintptr_t)g.workspace % 256 == 0 && g.workspace_nbytes >= p.bytes, "beam_select: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", p.bytes,
+                 g.workspace_nbytes);
+    if ((rc = paged_check_device(g.logits, "beam_select", "logits")) != B200_STATUS_SUCCESS) return rc;
+    if ((rc = paged_check_device(g.workspace, "beam_select", "the workspace")) != B200_STATUS_SUCCESS) return rc;
+    uint8_t *const ws = (uint8_t *)g.workspace;
+    SelectArgs a;
+    a.logits = (const uint8_t *)g.logits;
+    a.scores = g.scores;
+    a.done = g.done;
+    a.ld = g.logits_ld;
+    a.n_vocab = g.n_vocab;
+    a.n_beam = g.n_beam;
+    a.k = g.k;
+    a.chunks = (int)p.chunks;
+    a.end_token = g.end_token;
+    a.cand = (Cand *)(ws + p.cand);
+    a.count = (int *)(ws + p.count);
+    a.top = (float *)(ws + p.top);
+    a.sum = (double *)(ws + p.sum);
+    a.out_scores = g.out_scores;
+    a.out_tokens = g.out_tokens;
+    a.out_parents = g.out_parents;
+    const cudaStream_t s = (cudaStream_t)stream;
+    if (g.logits_type == B200_TYPE_F32) rc = launch_rows<float>(a, p, s);
+    else if (g.logits_type == B200_TYPE_F16) rc = launch_rows<__half>(a, p, s);
+    else rc = launch_rows<__nv_bfloat16>(a, p, s);
+    if (rc != B200_STATUS_SUCCESS) return rc;
+    const int64_t total = p.chunks * g.n_beam * g.k;
+    const int n_cached = (int)(total < BS_CACHE ? total : BS_CACHE);
+    return launch_pdl(beam_merge_kernel, dim3((unsigned)g.n_request), dim3(BS_MERGE_NT), (size_t)n_cached * 8, s, a, n_cached);
+}
+
+}  // extern "C"
