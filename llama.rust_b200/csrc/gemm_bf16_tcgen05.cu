@@ -43,6 +43,14 @@ bool cache_tile_map(CUtensorMap *map, const void *base, int64_t d, int64_t heads
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+bool paged_tile_map(CUtensorMap *map, CUtensorMapDataType type, const void *base, int64_t d, int64_t heads, int64_t page, int64_t n_pages, int64_t page_stride, int box_pos) {
+    encode_fn enc = tensor_map_encoder();
+    if (!enc) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)page, (cuuint64_t)n_pages}, strides[3] = {(cuuint64_t)d * 2, (cuuint64_t)(heads * d) * 2, (cuuint64_t)page_stride};
+    const cuuint32_t box[4] = {64, 1, (cuuint32_t)box_pos, 1}, es[4] = {1, 1, 1, 1};
+    return enc(map, type, 4, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 namespace {
 

@@ -1,0 +1,406 @@
+// The shared part of b200_prefix_attn: all rows of a group against the positions they share, on the tcgen05 tensor cores.
+//
+//   acc = sum_p w_p v_p,  sum = sum_p w_p,  w_p = exp2(scale log2(e) q k_p - m)       over the whole tiles of 128 positions that a row shares, per part
+//
+//   * A CTA takes up to 128 rows (sequence of the group, query head of the key head), or 256 as two blocks, and a part of the tiles.  Row r of a block is lane r of tensor memory.
+//   * K and V come in tiles of 128 positions by TMA, a box a page (or as much of a page as a tile holds), the pages' ids read a tile ahead; K is a K-major
+//     and V an MN-major B operand, so neither is transposed.  A page id out of range is loaded from behind the last page (zeros), and the part's rows are marked to be
+//     computed again without it.
+//   * Two groups of four softmax warps work in turn (as published with FlashAttention-4): with one block of rows they take the tiles alternately, each with
+//     an output of its own; with two blocks each has its block and both read every tile.  While one computes weights the tensor cores have the other's
+//     products.  A thread owns a row; weights go back into tensor memory over the scores they came from, as the A operand of the second product.
+//   * A row sees a tile as a whole or not at all, so that no score is masked one by one.
+//   * The output is rescaled only when a row's maximum grows by more than 2^8 over the one in use: the weights' rounding is relative, so nothing is lost.
+// Every wait is bounded; a wait that runs out raises the CTA's abort flag and the device error word, and its rows are marked so that none is stored.
+#include "attn_tcgen05.cuh"
+#include "prefix_attn.cuh"
+
+namespace b200 {
+
+namespace {
+
+constexpr int TC_M = 128, TC_N = PX_TILE, TC_THREADS = 384, TC_SM_WARP0 = 4, TC_SLOTS_MAX = 8;
+constexpr int TC_ERR_WAIT = 4;
+constexpr float TC_LAZY = 8.0f;   // log2 of the growth of a maximum that is let pass
+
+template <typename T, int D, bool TWO>
+struct TcCfg {
+    static constexpr int CHUNKS = D / 64;               // 64 elements = one 128-byte swizzled box
+    static constexpr int TILE = TC_N * D * 2, Q = TC_M * D * 2 * (TWO ? 2 : 1);
+    static constexpr int SLOTS = D == 128 ? (TWO ? 5 : 6) : TC_SLOTS_MAX;
+    static constexpr int SMEM = Q + SLOTS * TILE + 1024;
+    static constexpr uint32_t O_COL = 2 * TC_N;         // tensor memory: two score tiles, then two outputs
+    static constexpr uint32_t TYPES = sizeof(T) == 2 && !std::is_same<T, __half>::value ? (1u << 7) | (1u << 10) : 0u;   // A and B are BF16
+    static constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((uint32_t)(TC_N >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
+    static constexpr uint32_t IDESC_O = (1u << 4) | TYPES | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);   // B is MN-major
+};
+struct TcShared {
+    uint64_t full[TC_SLOTS_MAX], empty[TC_SLOTS_MAX];
+    uint64_t sfull[2], pready[2];                       // scores of a softmax group stand; its weights stand
+    uint64_t qready, done;
+    uint32_t tmem_base;
+    int abort_flag, n_tiles, bad;
+};
+struct TcArgs {
+    uint32_t wait_limit;
+    int mute;   // test hook: this tile's values are not asked for by the first CTA
+    int box;    // positions of a box
+};
+
+__device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int x, int head, int pos, int page, uint64_t *bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(pos), "r"(page),
+                 "r"(pa_smem(bar))
+                 : "memory");
+}
+
+template <typename T, int D, bool TWO>
+__global__ void __launch_bounds__(TC_THREADS, 1)
+prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefixArgs a, const TcArgs ta) {
+    using C = TcCfg<T, D, TWO>;
+    constexpr int ROWS = TWO ? 2 * TC_M : TC_M;
+    extern __shared__ uint8_t tc_raw[];
+    __shared__ TcShared sh;
+    const uint32_t q_s = (pa_smem(tc_raw) + 1023u) & ~1023u, kv_s = q_s + C::Q;
+    uint8_t *const q_g = tc_raw + (q_s - pa_smem(tc_raw));
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    volatile int *abort_flag = &sh.abort_flag;
+    int64_t id = blockIdx.x;
+    const int part = (int)(id % a.shared_parts); id /= a.shared_parts;
+    const int blk = (int)(id % a.shared_blocks); id /= a.shared_blocks;
+    const int hk = (int)(id % a.cache.n_head_kv), grp = (int)(id / a.cache.n_head_kv);
+
+    if (tid == 0) {
+        for (int i = 0; i < C::SLOTS; i++) {
+            pa_init(&sh.full[i], 1);
+            pa_init(&sh.empty[i], 1);
+        }
+        for (int g = 0; g < 2; g++) {
+            pa_init(&sh.sfull[g], 1);
+            pa_init(&sh.pready[g], 4);
+        }
+        pa_init(&sh.qready, 8);
+        pa_init(&sh.done, 1);
+        sh.abort_flag = 0;
+        sh.n_tiles = sh.bad = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pa_smem(&sh.tmem_base)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    pa_fence_before();
+    __syncthreads();
+    pa_fence_after();
+    const uint32_t tmem = sh.tmem_base;
+    pdl_wait();      // q, the cache rows of this step and the lengths come from earlier kernels
+    pdl_trigger();   // whoever starts now may count on these
+    // the group's rows: row x is sequence first + x / each, head hk * each + x % each
+    int first = a.group_first[grp], end = a.group_first[grp + 1];
+    const bool fits = prefix_group_fits(first, end, a.n_seq);
+    if (!fits) {
+        if (tid == 0) atomicExch(a.err, ERR_PAGED);
+        first = end = 0;
+    }
+    const int x0 = blk * ROWS, n_rows = min(end - first, a.served) * a.each - x0;   // may be negative
+    // the tiles that any of this CTA's rows sees, and this part's share of them
+    if (tid < ROWS && tid < n_rows) atomicMax(&sh.n_tiles, prefix_cover(a, first + (x0 + tid) / a.each) / PX_TILE);
+    __syncthreads();
+    const int capacity = (int)min(a.cache.table_ld << a.cache.page_log2 >> 7, (int64_t)0xffffff);
+    int n_all = sh.n_tiles;
+    if (n_all > capacity) {   // the own part reports it
+        n_all = capacity;
+    }
+    const int per = (n_all + a.shared_parts - 1) / a.shared_parts, t0 = min(part * per, n_all), n_tiles = min(per, n_all - t0);
+    const int steps = TWO ? 2 * n_tiles : n_tiles;
+
+    if (warp < TC_SM_WARP0) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        if (warp == 0 && n_tiles > 0) {
+            const int boxes = TC_N / ta.box, my_box = lane % boxes, my_chunk = lane / boxes;   // up to 8 boxes x 2 chunks
+            const bool mine = lane < boxes * C::CHUNKS;
+            const int32_t *const table = a.cache.tables + (int64_t)first * a.cache.table_ld;
+            const int page_mask = (1 << a.cache.page_log2) - 1;
+            // page id of this lane's box of a tile; what is out of range is read from behind the last page (zeros)
+            auto page_of = [&](int t) -> int {
+                if (!mine || t >= n_tiles) return 0;
+                const int32_t p = __ldg(table + (((int64_t)(t0 + t) * TC_N + my_box * ta.box) >> a.cache.page_log2));
+                if (p < 0 || p >= a.cache.n_pages) {
+                    atomicExch(a.err, ERR_PAGED);
+                    *(volatile int *)&sh.bad = 1;   // in front of this tile's arrival: the rows' last barrier comes behind it
+                    return (int)min(a.cache.n_pages, (int64_t)0x7fffffff);
+                }
+                return p;
+            };
+            int seq = 0;
+            bool ok = true;
+            const int mute = blockIdx.x == 0 ? ta.mute : -1;
+            auto load = [&](const CUtensorMap *map, int t, int page, bool ask) {
+                const int s = seq % C::SLOTS;
+                ok = ok && pa_wait(&sh.empty[s], ((uint32_t)(seq / C::SLOTS) & 1u) ^ 1u, abort_flag, ta.wait_limit);
+                if (!ok) return;
+                if (lane == 0) pa_expect(&sh.full[s], C::TILE);
+                __syncwarp();
+                if (mine && ask)
+                    tc_tma(kv_s + (uint32_t)(s * C::TILE + my_chunk * (TC_N * 128) + my_box * ta.box * 128), map, 64 * my_chunk, hk, ((t0 + t) * TC_N + my_box * ta.box) & page_mask, page, &sh.full[s]);
+                seq++;
+            };
+            // K 0, (K 1,) then V v and the next K, the order in which the products read them
+            constexpr int AHEAD = TWO ? 1 : 2;
+            int page[AHEAD + 1];
+#pragma unroll
+            for (int i = 0; i <= AHEAD; i++) page[i] = page_of(i);
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (i < n_tiles) load(&kmap, i, page[i], true);
+            for (int v = 0; v < n_tiles && ok; v++) {
+                const int next = page_of(v + AHEAD + 1);
+                load(&vmap, v, page[0], v != mute);
+                if (ok && v + AHEAD < n_tiles) load(&kmap, v + AHEAD, page[AHEAD], true);
+#pragma unroll
+                for (int i = 0; i < AHEAD; i++) page[i] = page[i + 1];
+                page[AHEAD] = next;
+            }
+            // a CTA that gives up still waits (bounded) for the copies it has in flight: a slot's last one
+            if (*abort_flag)
+                for (int q = seq > C::SLOTS ? seq - C::SLOTS : 0; q < seq; q++) pa_drain(&sh.full[q % C::SLOTS], (uint32_t)(q / C::SLOTS) & 1u, ta.wait_limit);
+        } else if (warp == 1 && n_tiles > 0) {
+            // the whole warp waits, one elected lane issues: descriptors then stay in uniform registers
+            const bool leader = pa_elect();
+            int seq = 0, k_slot = 0, v_slot = 0;
+            const uint64_t q_desc = pa_desc(q_s, 16), k_desc = pa_desc(kv_s, 16), v_desc = pa_desc(kv_s, TC_N * 128);
+            bool ok = pa_wait(&sh.qready, 0, abort_flag, ta.wait_limit);
+            auto arrived = [&](int *slot) {   // the next tile in the ring
+                *slot = seq % C::SLOTS;
+                ok = ok && pa_wait(&sh.full[*slot], (uint32_t)(seq / C::SLOTS) & 1u, abort_flag, ta.wait_limit);
+                seq++;
+            };
+            // scores of step n, for softmax group n % 2: over its former weights, whose product was issued before (products complete in order)
+            auto scores = [&](int n) {
+                const int g = n & 1;
+                if (!TWO || g == 0) arrived(&k_slot);
+                if (!ok) return;
+                pa_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ks++) {
+                        const uint32_t off = (uint32_t)((ks >> 2) * TC_M * 128 + (ks & 3) * 32) >> 4;
+                        pa_mma_ss(tmem + (uint32_t)(g * TC_N), q_desc + off + (uint32_t)(TWO ? g * (TC_M * D * 2 >> 4) : 0), k_desc + (uint32_t)(k_slot * (C::TILE >> 4)) + off, C::IDESC_S, ks > 0);
+                    }
+                    if (!TWO || g == 1) pa_commit(&sh.empty[k_slot]);
+                    pa_commit(&sh.sfull[g]);
+                }
+            };
+            for (int n = 0; n < 2 && n < steps && ok; n++) scores(n);
+            for (int n = 0; n < steps && ok; n++) {
+                const int g = n & 1, j = n >> 1;
+                if (!TWO || g == 0) arrived(&v_slot);
+                ok = ok && pa_wait(&sh.pready[g], (uint32_t)j & 1u, abort_flag, ta.wait_limit);
+                if (!ok) break;
+                pa_fence_after();
+                if (leader) {
+#pragma unroll
+                    for (int ks = 0; ks < TC_N / 16; ks++)
+                        pa_mma_ts(tmem + C::O_COL + (uint32_t)(g * D), tmem + (uint32_t)(g * TC_N + ks * 8), v_desc + (uint32_t)(v_slot * (C::TILE >> 4) + ks * 128), C::IDESC_O, j > 0 || ks > 0);
+                    if (!TWO || g == 1) pa_commit(&sh.empty[v_slot]);
+                }
+                if (n + 2 < steps) scores(n + 2);
+            }
+            if (leader) pa_commit(&sh.done);
+            // the operands and tensor memory stay until the products are through, whatever the other roles do
+            pa_drain(&sh.done, 0, ta.wait_limit);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int g = (warp - TC_SM_WARP0) >> 2, r = (warp & 3) * 32 + lane;   // softmax group, row of its block: a warp reaches the tensor-memory lanes of its number modulo 4
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t t_s = tmem + lanes + (uint32_t)(g * TC_N), t_o = tmem + lanes + C::O_COL + (uint32_t)(g * D);
+        const int x = (TWO ? g * TC_M : 0) + r;
+        const bool live = x < n_rows;
+        const int seq = first + (live ? (x0 + x) / a.each : 0), head = hk * a.each + (live ? (x0 + x) % a.each : 0);
+        const int64_t out = ((int64_t)seq * a.n_head + head) * (a.shared_parts + a.own_parts) + part;
+        const int my_tiles = live ? min(prefix_cover(a, seq) / PX_TILE, n_all) - t0 : 0;   // tiles of this part that the row sees
+        if (n_tiles > 0) {
+            // q into the swizzled K-major operand: a warp takes ROWS / 8 rows, a lane 8 bytes
+            constexpr int LANES = D / 4, PER = 32 / LANES;   // lanes of a row, rows at a time
+            constexpr int RW = ROWS / 8;
+            const int e = lane % LANES, c = e >> 4, u = (e & 15) >> 1;
+#pragma unroll 8
+            for (int h = 0; h < RW; h += PER) {
+                const int y = (warp - TC_SM_WARP0) * RW + h + lane / LANES, yb = y % TC_M;
+                uint2 w = make_uint2(0u, 0u);
+                if (y < n_rows) w = *(const uint2 *)(a.q + (int64_t)(first + (x0 + y) / a.each) * a.q_nb1 + (int64_t)(hk * a.each + (x0 + y) % a.each) * a.q_nb2 + 8 * e);
+                *(uint2 *)(q_g + (y / TC_M) * (TC_M * D * 2) + c * (TC_M * 128) + (yb >> 3) * 1024 + (yb & 7) * 128 + ((u ^ (yb & 7)) << 4) + (e & 1) * 8) = w;
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) pa_arrive(&sh.qready);
+        }
+        float m = -INFINITY, l = 0.0f;   // the maximum in use (log2 units) and the sum of the weights under it
+        const bool warp_live = __any_sync(0xffffffffu, live);
+        const int turns = TWO ? n_tiles : (n_tiles + 1 - g) / 2;
+        for (int j = 0; j < turns; j++) {
+            if (!pa_wait(&sh.sfull[g], (uint32_t)j & 1u, abort_flag, ta.wait_limit)) break;
+            if (warp_live) {
+                pa_fence_after();
+                const bool sees = (TWO ? j : 2 * j + g) < my_tiles;
+                uint32_t s[TC_N];
+#pragma unroll
+                for (int c = 0; c < TC_N; c += 32) pa_ld32(s + c, t_s + (uint32_t)c);
+                pa_wait_ld();
+                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                // of the raw scores the largest, under a negative scale the smallest
+                const float sc = a.scale_log2;
+                if (sc >= 0.0f) {
+#pragma unroll
+                    for (int c = 0; c < TC_N; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[c + e]), __uint_as_float(s[c + 4 + e])));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < TC_N; c += 4)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], -__uint_as_float(s[c + e]));
+                }
+                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                top = top == -INFINITY ? -INFINITY : top * fabsf(sc);
+                top = sees ? fmaxf(m, top) : m;
+                if (j == 0) {
+                    m = top;
+                } else {
+                    const bool grow = top > m + TC_LAZY;   // also when nothing was seen before
+                    if (__any_sync(0xffffffffu, grow)) {
+                        // the group's former product is complete: the scores that were waited for were issued behind it
+                        const float al = grow ? pa_ex2(m - top) : 1.0f;
+                        if (grow) m = top;
+                        l *= al;
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            pa_ld32(o, t_o + (uint32_t)c);
+                            pa_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+                            pa_st32(t_o + (uint32_t)c, o);
+                        }
+                        pa_wait_st();
+                    }
+                }
+                const float sub = !sees ? INFINITY : m == -INFINITY ? 0.0f : m;   // a row that does not see the tile: weights of zero
+                uint64_t ps[2] = {0, 0};   // two running sums each
+                const uint64_t sc2 = pa_pair(sc, sc), sub2 = pa_pair(-sub, -sub);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int c = 0; c < 32; c++) {
+                        const float2 y = pa_split(pa_fma2(pa_pair(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1])), sc2, sub2));
+                        const float e0 = pa_ex2(y.x), e1 = pa_ex2(y.y);
+                        p[c] = paged_pack<T>(e0, e1);
+                        ps[c & 1] = pa_add2(ps[c & 1], pa_pair(e0, e1));
+                    }
+                    if (!sees) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++) p[c] = 0u;   // whatever the scores were
+                    }
+                    pa_st32(t_s + (uint32_t)(32 * h), p);
+                }
+                const float2 p0 = pa_split(ps[0]), p1 = pa_split(ps[1]);
+                if (sees) l += (p0.x + p1.x) + (p0.y + p1.y);
+                pa_wait_st();
+                pa_fence_before();
+            }
+            __syncwarp();
+            if (lane == 0) pa_arrive(&sh.pready[g]);
+        }
+        if (l != l) m = fmaxf(m, 0.0f);   // a NaN score is no maximum, but the row has seen it
+        if (n_tiles == 0) {
+            if (live && (TWO || g == 0)) a.ml[out] = make_float2(-INFINITY, 0.0f);
+        } else {
+            const bool finished = __all_sync(0xffffffffu, pa_wait(&sh.done, 0, abort_flag, ta.wait_limit) && !*abort_flag);
+            pa_fence_after();
+            float wa = 1.0f, wb = 0.0f;
+            bool ina = m != -INFINITY, inb = false;
+            int c0 = 0, c1 = D;
+            if (!TWO) {   // the two groups' outputs under their common maximum, half the channels each
+                float2 *const ml = (float2 *)(q_g + C::Q);   // [2][TC_M] in the first slot: its last product is through, or nothing of it will be stored
+                ml[g * TC_M + r] = make_float2(m, l);
+                asm volatile("bar.sync 1, 256;" ::: "memory");
+                const float2 la = ml[r], lb = ml[TC_M + r];
+                const float ma = la.x, mb = lb.x;
+                m = fmaxf(ma, mb);
+                ina = ma != -INFINITY;   // no output where the group had no tile or the row saw none of them
+                inb = mb != -INFINITY;
+                wa = ina ? pa_ex2(ma - m) : 0.0f;
+                wb = inb ? pa_ex2(mb - m) : 0.0f;
+                l = (ina ? wa * la.y : 0.0f) + (inb ? wb * lb.y : 0.0f);
+                c0 = g * (D / 2);
+                c1 = c0 + D / 2;
+            }
+            if (live && c0 == 0) a.ml[out] = !finished ? make_float2(NAN, NAN) : *(volatile int *)&sh.bad ? make_float2(NAN, 0.0f) : make_float2(m, l);
+            if (finished && warp_live) {
+                float *const dst = a.acc + out * D;
+#pragma unroll 1
+                for (int c = c0; c < c1; c += 32) {
+                    uint32_t u[32], v[TWO ? 1 : 32];
+                    pa_ld32(u, tmem + lanes + C::O_COL + (uint32_t)((TWO ? g * D : 0) + c));
+                    if constexpr (!TWO) pa_ld32(v, tmem + lanes + C::O_COL + (uint32_t)(D + c));
+                    pa_wait_ld();
+                    if (live && m != -INFINITY) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            float z = __uint_as_float(u[e]);
+                            if constexpr (!TWO) z = (ina ? wa * z : 0.0f) + (inb ? wb * __uint_as_float(v[e]) : 0.0f);
+                            u[e] = __float_as_uint(z);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c + e), "r"(u[e]), "r"(u[e + 1]), "r"(u[e + 2]), "r"(u[e + 3]), "r"(u[e + 4]), "r"(u[e + 5]), "r"(u[e + 6]),
+                                         "r"(u[e + 7])
+                                         : "memory");
+                    }
+                }
+            }
+        }
+        pa_fence_before();
+    }
+    __syncthreads();
+    pa_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    if (*abort_flag && tid == 0) atomicExch(a.err, TC_ERR_WAIT);
+}
+
+template <typename T, int D, bool TWO>
+int launch(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
+    using C = TcCfg<T, D, TWO>;
+    TcArgs ta;
+    attn_wait_hook(&ta.wait_limit, &ta.mute);
+    const int page = 1 << a.cache.page_log2;
+    ta.box = page < TC_N ? page : TC_N;
+    CUtensorMap km, vm;
+    B200_REQUIRE(paged_tile_map(&km, type, a.cache.k, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box) &&
+                     paged_tile_map(&vm, type, a.cache.v, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box),
+                 "prefix_attn: tensor maps over %lld pages of %d positions refused", (long long)a.cache.n_pages, page);
+    B200_CUDA(cudaFuncSetAttribute(prefix_shared_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    // the warps' register shares come out of what the block is launched with
+    cudaFuncAttributes fa;
+    B200_CUDA(cudaFuncGetAttributes(&fa, prefix_shared_kernel<T, D, TWO>));
+    B200_REQUIRE(fa.numRegs * TC_THREADS >= 64 * TC_SM_WARP0 * 32 + 216 * (TC_THREADS - TC_SM_WARP0 * 32), "prefix_attn: a build with %d registers a thread cannot share them out", fa.numRegs);
+    const int64_t ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts;
+    return launch_pdl(prefix_shared_kernel<T, D, TWO>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
+}
+
+}  // namespace
+
+int prefix_shared_rows(int64_t rows) { return rows > TC_M ? 2 * TC_M : TC_M; }
+
+int launch_prefix_shared(const PrefixArgs &a, int type, cudaStream_t s) {
+    const bool two = prefix_shared_rows((int64_t)a.served * a.each) == 2 * TC_M;
+    if (type == B200_TYPE_F16) {
+        if (a.cache.d == 128) return two ? launch<__half, 128, true>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s) : launch<__half, 128, false>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s);
+        return two ? launch<__half, 64, true>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s) : launch<__half, 64, false>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s);
+    }
+    if (a.cache.d == 128) return two ? launch<__nv_bfloat16, 128, true>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s) : launch<__nv_bfloat16, 128, false>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s);
+    return two ? launch<__nv_bfloat16, 64, true>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s) : launch<__nv_bfloat16, 64, false>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s);
+}
+
+}  // namespace b200
