@@ -16,13 +16,16 @@ namespace {
 
 constexpr int PX_BM = 16, PX_BN = 64, PX_WARPS = 4, PX_NT = PX_WARPS * 32;
 constexpr int PX_MAX_PARTS = 64;   // of the shared positions, and of a row's own
+template <int D>
+constexpr int PX_STAGES = D == 128 ? 2 : 4;   // 64 KB of tiles under way or at work: a CTA then fits an SM beside one of the shared part's (161 KB, and 128 registers a thread each)
 
 __device__ __forceinline__ uint32_t px_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void px_cp16(void *dst, const void *src, bool there) {   // zeros where there is nothing to read
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(px_smem(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 __device__ __forceinline__ void px_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void px_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void px_wait_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void px_ldsm(uint32_t (&r)[4], const void *p) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(px_smem(p)));
 }
@@ -77,10 +80,10 @@ __device__ __forceinline__ int prefix_first(const PrefixArgs &a, int s, bool *se
 // 16 w .. + 15 of every tile of 64 (its own maximum and sum), the four are joined at the end.  Positions that the sequence does not see are zeros in
 // shared memory, whatever the page holds.
 template <typename T, int D>
-__global__ void __launch_bounds__(PX_NT) prefix_own_kernel(const PrefixArgs a, bool after_shared) {
-    constexpr int PITCH = D * 2 + 16, KS = D / 16, DB = D / 8, TILE = PX_BN * PITCH;
-    extern __shared__ __align__(16) unsigned char smem[];   // K [2][PX_BN][PITCH], V the same
-    __shared__ int64_t cell_of[2][PX_BN];                   // byte offset of a tile's positions, -1: not there
+__global__ void __launch_bounds__(PX_NT, 4) prefix_own_kernel(const PrefixArgs a, bool after_shared) {
+    constexpr int ROW = D * 2, KS = D / 16, DB = D / 8, TILE = PX_BN * ROW, NST = PX_STAGES<D>;
+    extern __shared__ __align__(128) unsigned char smem[];   // K [NST][PX_BN][ROW], V the same; 16-byte piece u of row r lies at u ^ (r % 8)
+    __shared__ int64_t cell_of[NST][PX_BN];                  // byte offset of a tile's positions, -1: not there
     __shared__ float wm[PX_WARPS][PX_BM], wl[PX_WARPS][PX_BM];
     pdl_trigger();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -101,6 +104,7 @@ __global__ void __launch_bounds__(PX_NT) prefix_own_kernel(const PrefixArgs a, b
     const int64_t head = (int64_t)hk * D * 2;
     // a thread's pieces of a tile: 16 bytes tid % PIECES of rows tid / PIECES + RSTEP j
     constexpr int PIECES = D / 8, RSTEP = PX_NT / PIECES, PASSES = PX_BN / RSTEP;
+    static_assert(RSTEP % 8 == 0, "a thread's rows have one place for their piece");
     auto look_up = [&](int tile) -> int64_t {   // the threads of the first two warps: a position each
         const int p = p0 + tile * PX_BN + tid;
         if (tid >= PX_BN || tile >= n_walk || p >= end) return -1;
@@ -109,26 +113,30 @@ __global__ void __launch_bounds__(PX_NT) prefix_own_kernel(const PrefixArgs a, b
         return at;
     };
     auto stage = [&](int buf) {
-        unsigned char *const kd = smem + buf * TILE + (tid / PIECES) * PITCH + (tid % PIECES) * 16, *const vd = kd + 2 * TILE;
+        unsigned char *const kd = smem + buf * TILE + (tid / PIECES) * ROW + (((tid % PIECES) ^ (tid / PIECES & 7)) << 4), *const vd = kd + NST * TILE;
 #pragma unroll
         for (int j = 0; j < PASSES; j++) {
             const int64_t at = cell_of[buf][tid / PIECES + j * RSTEP];
             const int64_t from = (at < 0 ? 0 : at + head) + (tid % PIECES) * 16;
-            px_cp16(kd + j * RSTEP * PITCH, a.cache.k + from, at >= 0);
-            px_cp16(vd + j * RSTEP * PITCH, a.cache.v + from, at >= 0);
+            px_cp16(kd + j * RSTEP * ROW, a.cache.k + from, at >= 0);
+            px_cp16(vd + j * RSTEP * ROW, a.cache.v + from, at >= 0);
         }
-        px_commit();
     };
     {
-        const int64_t c0 = look_up(0), c1 = look_up(1);
+        int64_t c[NST];
+#pragma unroll
+        for (int i = 0; i < NST; i++) c[i] = look_up(i);
         if (tid < PX_BN) {
-            cell_of[0][tid] = c0;
-            cell_of[1][tid] = c1;
+#pragma unroll
+            for (int i = 0; i < NST; i++) cell_of[i][tid] = c[i];
         }
     }
     __syncthreads();
-    if (n_walk > 0) stage(0); else px_commit();
-    if (n_walk > 1) stage(1); else px_commit();
+#pragma unroll
+    for (int i = 0; i < NST; i++) {
+        if (i < n_walk) stage(i);
+        px_commit();
+    }
     const int r_a = lane >> 2, r_b = r_a + 8;   // this thread's rows
     uint32_t qf[KS][4];
     {
@@ -147,22 +155,22 @@ __global__ void __launch_bounds__(PX_NT) prefix_own_kernel(const PrefixArgs a, b
 #pragma unroll
     for (int j = 0; j < DB; j++) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.0f;
     float m_a = -INFINITY, m_b = -INFINITY, l_a = 0.0f, l_b = 0.0f;
-    const int k_row = (lane & 7) + ((lane >> 4) << 3), k_col = ((lane >> 3) & 1) * 16;
-    const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_col = (lane >> 4) * 16;
+    const int k_row = (lane & 7) + ((lane >> 4) << 3), k_piece = (lane >> 3) & 1;
+    const int v_row = (lane & 7) + (((lane >> 3) & 1) << 3), v_piece = lane >> 4, turn = lane & 7;   // rows' places modulo 8
     const int pw = 16 * warp;
     for (int it = 0; it < n_walk; it++) {
-        const int buf = it & 1;
-        const int64_t next = look_up(it + 2);
-        px_wait_but_one();
+        const int buf = it % NST;
+        const int64_t next = look_up(it + NST);
+        px_wait_but<NST - 1>();
         __syncthreads();
-        const unsigned char *const kt = smem + buf * TILE, *const vt = kt + 2 * TILE;
+        const unsigned char *const kt = smem + buf * TILE + (pw + k_row) * ROW, *const vt = smem + (NST + buf) * TILE + (pw + v_row) * ROW;
         float sc[2][4];
 #pragma unroll
         for (int n = 0; n < 2; n++) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.0f;
 #pragma unroll
         for (int st = 0; st < KS; st++) {
             uint32_t b[4];
-            px_ldsm(b, kt + (pw + k_row) * PITCH + st * 32 + k_col);
+            px_ldsm(b, kt + (((2 * st + k_piece) ^ turn) << 4));
             px_mma<T>(sc[0], qf[st], b[0], b[1]);
             px_mma<T>(sc[1], qf[st], b[2], b[3]);
         }
@@ -201,14 +209,15 @@ __global__ void __launch_bounds__(PX_NT) prefix_own_kernel(const PrefixArgs a, b
 #pragma unroll
         for (int e = 0; e < DB; e += 2) {
             uint32_t b[4];
-            px_ldsm_t(b, vt + (pw + v_row) * PITCH + e * 16 + v_col);
+            px_ldsm_t(b, vt + (((e + v_piece) ^ turn) << 4));
             px_mma<T>(o[e], pf, b[0], b[1]);
             px_mma<T>(o[e + 1], pf, b[2], b[3]);
         }
         __syncthreads();   // everyone is done with this buffer
         if (tid < PX_BN) cell_of[buf][tid] = next;
         __syncthreads();
-        if (it + 2 < n_walk) stage(buf); else px_commit();
+        if (it + NST < n_walk) stage(buf);
+        px_commit();
     }
     // the four warps joined
     l_a += __shfl_xor_sync(0xffffffffu, l_a, 1); l_a += __shfl_xor_sync(0xffffffffu, l_a, 2);
@@ -410,7 +419,7 @@ int prefix_plan(const b200_prefix_attn_args &g, PrefixPlan *p) {
     }
     a.own_blocks = (a.each + PX_BM - 1) / PX_BM;
     const int64_t own_items = (int64_t)g.n_seq * kv * a.own_blocks, own = g.max_len - shared_tiles * PX_TILE;
-    a.own_parts = parts(own_items, own > PX_BN ? (own + PX_BN - 1) / PX_BN : 1, sms * (g.cache.d == 128 ? 3 : 4));
+    a.own_parts = parts(own_items, own > PX_BN ? (own + PX_BN - 1) / PX_BN : 1, sms * 3);
     B200_REQUIRE(own_items * a.own_parts < 0x7fffffffLL, "prefix_attn: too many rows for one launch");
     p->rows = (int64_t)g.n_seq * g.n_head;
     const int64_t slots = p->rows * (a.shared_parts + a.own_parts);
@@ -422,7 +431,7 @@ int prefix_plan(const b200_prefix_attn_args &g, PrefixPlan *p) {
 template <typename T, int D>
 int launch_prefix(const PrefixPlan &p, int type, cudaStream_t s) {
     const PrefixArgs &a = p.a;
-    constexpr int SMEM = 4 * PX_BN * (D * 2 + 16);
+    constexpr int SMEM = 2 * PX_STAGES<D> * PX_BN * D * 2;
     int rc = a.shared_parts ? launch_prefix_shared(a, type, s) : B200_STATUS_SUCCESS;
     if (rc != B200_STATUS_SUCCESS) return rc;
     const int64_t ctas = (int64_t)a.n_seq * a.cache.n_head_kv * a.own_blocks * a.own_parts;

@@ -10,7 +10,8 @@
 //     an output of its own; with two blocks each has its block and both read every tile.  While one computes weights the tensor cores have the other's
 //     products.  A thread owns a row; weights go back into tensor memory over the scores they came from, as the A operand of the second product.
 //   * A row sees a tile as a whole or not at all, so that no score is masked one by one.
-//   * The output is rescaled only when a row's maximum grows by more than 2^8 over the one in use: the weights' rounding is relative, so nothing is lost.
+//   * A tile's weights are taken under the maximum in use without a look at its scores; only where their sum exceeds 2^12 (or the row has seen nothing yet) are they taken
+//     again under the tile's own maximum, and the output rescaled: the weights' rounding is relative, so nothing is lost.
 // Every wait is bounded; a wait that runs out raises the CTA's abort flag and the device error word, and its rows are marked so that none is stored.
 #include "attn_tcgen05.cuh"
 #include "prefix_attn.cuh"
@@ -20,15 +21,17 @@ namespace b200 {
 namespace {
 
 constexpr int TC_M = 128, TC_N = PX_TILE, TC_THREADS = 384, TC_SM_WARP0 = 4, TC_SLOTS_MAX = 8;
+constexpr int TC_REGS = 128, TC_FEW_REGS = 40, TC_MANY_REGS = 168;   // a thread's at launch, then of the loading and of the softmax warps
 constexpr int TC_ERR_WAIT = 4;
-constexpr float TC_LAZY = 8.0f;   // log2 of the growth of a maximum that is let pass
+constexpr float TC_MOST = 4096.0f;   // sum of a tile's weights up to which the maximum in use is kept
+static_assert(TC_FEW_REGS * TC_SM_WARP0 * 32 + TC_MANY_REGS * (TC_THREADS - TC_SM_WARP0 * 32) <= TC_REGS * TC_THREADS, "register shares");
 
 template <typename T, int D, bool TWO>
 struct TcCfg {
     static constexpr int CHUNKS = D / 64;               // 64 elements = one 128-byte swizzled box
     static constexpr int TILE = TC_N * D * 2, Q = TC_M * D * 2 * (TWO ? 2 : 1);
-    static constexpr int SLOTS = D == 128 ? (TWO ? 5 : 6) : TC_SLOTS_MAX;
-    static constexpr int SMEM = Q + SLOTS * TILE + 1024;
+    static constexpr int SLOTS = D == 128 ? (TWO ? 3 : 4) : TC_SLOTS_MAX;
+    static constexpr int SMEM = Q + SLOTS * TILE + 256;   // the barriers behind the operands: nothing is static, so that the operands begin where shared memory does
     static constexpr uint32_t O_COL = 2 * TC_N;         // tensor memory: two score tiles, then two outputs
     static constexpr uint32_t TYPES = sizeof(T) == 2 && !std::is_same<T, __half>::value ? (1u << 7) | (1u << 10) : 0u;   // A and B are BF16
     static constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((uint32_t)(TC_N >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
@@ -53,15 +56,43 @@ __device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int
                  : "memory");
 }
 
+// Two powers of two.  Of the exponentials three in eight are computed by multiply-adds, so that the special function units (16 a clock and SM, 1024 clocks a
+// tile) and the others are done at about the same time: y = n + r with |r| <= 1/2, the polynomial is the relative minimax one of 2^r of degree 4 (by
+// Remez' exchange, 2.7e-6), n goes into the exponent.  Below 2^-126 it stays there.
+__device__ __forceinline__ float2 tc_ex2_units(uint64_t y) {
+    const float2 x = pa_split(y);
+    return make_float2(pa_ex2(x.x), pa_ex2(x.y));
+}
+__device__ __forceinline__ float2 tc_ex2_pair(uint64_t y) {
+    float2 x = pa_split(y);
+    x.x = fmaxf(x.x, -126.0f);
+    x.y = fmaxf(x.y, -126.0f);
+    const uint64_t v = pa_pair(x.x, x.y), big = pa_pair(12582912.0f, 12582912.0f), neg = pa_pair(-1.0f, -1.0f);   // 1.5 * 2^23: the sum's last bit is 1
+    const uint64_t t = pa_add2(v, big), r = pa_fma2(pa_add2(t, pa_pair(-12582912.0f, -12582912.0f)), neg, v);
+    uint64_t q = pa_pair(9.570102015e-03f, 9.570102015e-03f);
+    q = pa_fma2(q, r, pa_pair(5.591786031e-02f, 5.591786031e-02f));
+    q = pa_fma2(q, r, pa_pair(2.402474482e-01f, 2.402474482e-01f));
+    q = pa_fma2(q, r, pa_pair(6.931218147e-01f, 6.931218147e-01f));
+    q = pa_fma2(q, r, pa_pair(9.999992614e-01f, 9.999992614e-01f));
+    const float2 f = pa_split(q), n = pa_split(t);
+    return make_float2(__uint_as_float(__float_as_uint(f.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(f.y) + (__float_as_uint(n.y) << 23)));
+}
+
 template <typename T, int D, bool TWO>
-__global__ void __launch_bounds__(TC_THREADS, 1)
+__global__ void __maxnreg__(TC_REGS)
 prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefixArgs a, const TcArgs ta) {
     using C = TcCfg<T, D, TWO>;
     constexpr int ROWS = TWO ? 2 * TC_M : TC_M;
-    extern __shared__ uint8_t tc_raw[];
-    __shared__ TcShared sh;
-    const uint32_t q_s = (pa_smem(tc_raw) + 1023u) & ~1023u, kv_s = q_s + C::Q;
-    uint8_t *const q_g = tc_raw + (q_s - pa_smem(tc_raw));
+    extern __shared__ __align__(1024) uint8_t tc_raw[];
+    static_assert(sizeof(TcShared) <= 256, "barriers");
+    TcShared &sh = *(TcShared *)(tc_raw + C::Q + C::SLOTS * C::TILE);
+    const uint32_t q_s = pa_smem(tc_raw), kv_s = q_s + C::Q;
+    uint8_t *const q_g = tc_raw;
+    if (q_s & 1023u) {   // the swizzle counts in 1024 bytes
+        pdl_wait();
+        if (threadIdx.x == 0) atomicExch(a.err, TC_ERR_WAIT);
+        return;
+    }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     volatile int *abort_flag = &sh.abort_flag;
     int64_t id = blockIdx.x;
@@ -114,7 +145,7 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     const int steps = TWO ? 2 * n_tiles : n_tiles;
 
     if (warp < TC_SM_WARP0) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_FEW_REGS));
         if (warp == 0 && n_tiles > 0) {
             const int boxes = TC_N / ta.box, my_box = lane % boxes, my_chunk = lane / boxes;   // up to 8 boxes x 2 chunks
             const bool mine = lane < boxes * C::CHUNKS;
@@ -210,7 +241,7 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             pa_drain(&sh.done, 0, ta.wait_limit);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TC_MANY_REGS));
         const int g = (warp - TC_SM_WARP0) >> 2, r = (warp & 3) * 32 + lane;   // softmax group, row of its block: a warp reaches the tensor-memory lanes of its number modulo 4
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lanes + (uint32_t)(g * TC_N), t_o = tmem + lanes + C::O_COL + (uint32_t)(g * D);
@@ -220,17 +251,19 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const int64_t out = ((int64_t)seq * a.n_head + head) * (a.shared_parts + a.own_parts) + part;
         const int my_tiles = live ? min(prefix_cover(a, seq) / PX_TILE, n_all) - t0 : 0;   // tiles of this part that the row sees
         if (n_tiles > 0) {
-            // q into the swizzled K-major operand: a warp takes ROWS / 8 rows, a lane 8 bytes
-            constexpr int LANES = D / 4, PER = 32 / LANES;   // lanes of a row, rows at a time
-            constexpr int RW = ROWS / 8;
-            const int e = lane % LANES, c = e >> 4, u = (e & 15) >> 1;
-#pragma unroll 8
+            // q into the swizzled K-major operand, zeros behind the last row: a warp takes ROWS / 8 rows, a lane 16 bytes at a time, all under way at once (row by row
+            // through registers this took 14 us of a launch)
+            constexpr int LANES = D / 8, PER = 32 / LANES, RW = ROWS / 8;   // lanes of a row, rows at a time
+            const int e = lane % LANES, c = e >> 3, u = e & 7;
+#pragma unroll
             for (int h = 0; h < RW; h += PER) {
-                const int y = (warp - TC_SM_WARP0) * RW + h + lane / LANES, yb = y % TC_M;
-                uint2 w = make_uint2(0u, 0u);
-                if (y < n_rows) w = *(const uint2 *)(a.q + (int64_t)(first + (x0 + y) / a.each) * a.q_nb1 + (int64_t)(hk * a.each + (x0 + y) % a.each) * a.q_nb2 + 8 * e);
-                *(uint2 *)(q_g + (y / TC_M) * (TC_M * D * 2) + c * (TC_M * 128) + (yb >> 3) * 1024 + (yb & 7) * 128 + ((u ^ (yb & 7)) << 4) + (e & 1) * 8) = w;
+                const int y = (warp - TC_SM_WARP0) * RW + h + lane / LANES, yb = y % TC_M, row = x0 + (y < n_rows ? y : 0), i = row / a.each;
+                const uint8_t *const src = a.q + (int64_t)(first + i) * a.q_nb1 + (int64_t)(hk * a.each + row - i * a.each) * a.q_nb2 + 16 * e;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_s + (uint32_t)((y / TC_M) * (TC_M * D * 2) + c * (TC_M * 128) + (yb >> 3) * 1024 + (yb & 7) * 128 + ((u ^ (yb & 7)) << 4))),
+                             "l"(src), "r"(y < n_rows ? 16 : 0)
+                             : "memory");
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) pa_arrive(&sh.qready);
@@ -243,69 +276,66 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
             if (warp_live) {
                 pa_fence_after();
                 const bool sees = (TWO ? j : 2 * j + g) < my_tiles;
-                uint32_t s[TC_N];
-#pragma unroll
-                for (int c = 0; c < TC_N; c += 32) pa_ld32(s + c, t_s + (uint32_t)c);
-                pa_wait_ld();
-                float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                // of the raw scores the largest, under a negative scale the smallest
                 const float sc = a.scale_log2;
-                if (sc >= 0.0f) {
+                uint32_t p[TC_N / 2];
+                // the weights under the maximum in use; where their sum says that it has grown too much, and where there is none yet, once more under the tile's own
+                bool anew = __any_sync(0xffffffffu, sees && m == -INFINITY);
+                for (;;) {
+                    uint32_t s[TC_N];
 #pragma unroll
-                    for (int c = 0; c < TC_N; c += 8)
+                    for (int c = 0; c < TC_N; c += 32) pa_ld32(s + c, t_s + (uint32_t)c);
+                    pa_wait_ld();
+                    if (anew) {
+                        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        const float sign = sc < 0.0f ? -1.0f : 1.0f;   // under a negative scale the smallest score is the largest
 #pragma unroll
-                        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], fmaxf(__uint_as_float(s[c + e]), __uint_as_float(s[c + 4 + e])));
-                } else {
+                        for (int c = 0; c < TC_N; c += 4)
 #pragma unroll
-                    for (int c = 0; c < TC_N; c += 4)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], -__uint_as_float(s[c + e]));
-                }
-                float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                top = top == -INFINITY ? -INFINITY : top * fabsf(sc);
-                top = sees ? fmaxf(m, top) : m;
-                if (j == 0) {
-                    m = top;
-                } else {
-                    const bool grow = top > m + TC_LAZY;   // also when nothing was seen before
-                    if (__any_sync(0xffffffffu, grow)) {
-                        // the group's former product is complete: the scores that were waited for were issued behind it
-                        const float al = grow ? pa_ex2(m - top) : 1.0f;
-                        if (grow) m = top;
+                            for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], sign * __uint_as_float(s[c + e]));
+                        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                        top = top == -INFINITY ? -INFINITY : top * fabsf(sc);
+                        const float al = sees && top > m ? pa_ex2(m - top) : 1.0f;
+                        if (sees) m = fmaxf(m, top);
                         l *= al;
+                        if (j > 0 && __any_sync(0xffffffffu, al != 1.0f)) {
+                            // the group's former product is complete: the scores that were waited for were issued behind it
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            pa_ld32(o, t_o + (uint32_t)c);
-                            pa_wait_ld();
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                pa_ld32(o, t_o + (uint32_t)c);
+                                pa_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
-                            pa_st32(t_o + (uint32_t)c, o);
+                                for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * al);
+                                pa_st32(t_o + (uint32_t)c, o);
+                            }
+                            pa_wait_st();
                         }
-                        pa_wait_st();
                     }
+                    uint64_t ps[2] = {0, 0};   // two running sums each
+                    const float sub = m == -INFINITY ? 0.0f : -m;
+                    const uint64_t sc2 = pa_pair(sc, sc), sub2 = pa_pair(sub, sub);
+#pragma unroll
+                    for (int c = 0; c < TC_N / 2; c++) {
+                        const uint64_t y = pa_fma2(pa_pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, sub2);
+                        const float2 e = (c * 3) % 8 < 3 ? tc_ex2_pair(y) : tc_ex2_units(y);
+                        p[c] = paged_pack<T>(e.x, e.y);
+                        ps[c & 1] = pa_add2(ps[c & 1], pa_pair(e.x, e.y));
+                    }
+                    const float2 p0 = pa_split(ps[0]), p1 = pa_split(ps[1]);
+                    const float sum = (p0.x + p1.x) + (p0.y + p1.y);
+                    if (anew || !__any_sync(0xffffffffu, sees && !(sum <= TC_MOST))) {
+                        if (sees && m > -INFINITY) l += sum;
+                        else if (sees && sum != sum) l = sum;   // NaN scores alone
+                        break;
+                    }
+                    anew = true;
                 }
-                const float sub = !sees ? INFINITY : m == -INFINITY ? 0.0f : m;   // a row that does not see the tile: weights of zero
-                uint64_t ps[2] = {0, 0};   // two running sums each
-                const uint64_t sc2 = pa_pair(sc, sc), sub2 = pa_pair(-sub, -sub);
+                if (!sees || m == -INFINITY) {   // weights of zero, whatever the scores were
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int c = 0; c < 32; c++) {
-                        const float2 y = pa_split(pa_fma2(pa_pair(__uint_as_float(s[64 * h + 2 * c]), __uint_as_float(s[64 * h + 2 * c + 1])), sc2, sub2));
-                        const float e0 = pa_ex2(y.x), e1 = pa_ex2(y.y);
-                        p[c] = paged_pack<T>(e0, e1);
-                        ps[c & 1] = pa_add2(ps[c & 1], pa_pair(e0, e1));
-                    }
-                    if (!sees) {
-#pragma unroll
-                        for (int c = 0; c < 32; c++) p[c] = 0u;   // whatever the scores were
-                    }
-                    pa_st32(t_s + (uint32_t)(32 * h), p);
+                    for (int c = 0; c < TC_N / 2; c++) p[c] = 0u;
                 }
-                const float2 p0 = pa_split(ps[0]), p1 = pa_split(ps[1]);
-                if (sees) l += (p0.x + p1.x) + (p0.y + p1.y);
+                pa_st32(t_s, p);
+                pa_st32(t_s + 32u, p + 32);
                 pa_wait_st();
                 pa_fence_before();
             }
@@ -384,7 +414,7 @@ int launch(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
     // the warps' register shares come out of what the block is launched with
     cudaFuncAttributes fa;
     B200_CUDA(cudaFuncGetAttributes(&fa, prefix_shared_kernel<T, D, TWO>));
-    B200_REQUIRE(fa.numRegs * TC_THREADS >= 64 * TC_SM_WARP0 * 32 + 216 * (TC_THREADS - TC_SM_WARP0 * 32), "prefix_attn: a build with %d registers a thread cannot share them out", fa.numRegs);
+    B200_REQUIRE(fa.numRegs >= TC_REGS, "prefix_attn: a build with %d registers a thread cannot share them out", fa.numRegs);
     const int64_t ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts;
     return launch_pdl(prefix_shared_kernel<T, D, TWO>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
 }
