@@ -18,8 +18,9 @@ struct PrefixArgs {
     int n_seq, n_head, n_group, each;         // each: query heads of a key head
     int served;                               // sequences of a group that the shared part takes; further ones read their shared positions with their own
     int shared_parts, shared_blocks;          // CTAs that a (group, key head)'s positions and rows are dealt to
-    int own_parts, own_blocks;                // the same of a (sequence, key head)
-    float2 *ml;                               // [row][part]: maximum (log2 units), sum; the shared parts first
+    int own_parts, own_blocks;                // parts and blocks of 16 rows of a (sequence, key head)
+    int own_ctas;                             // CTAs that walk them
+    float2 *ml;                               // [row][part]: maximum (log2 units), sum; the shared parts first, then PX_WARPS for each of a row's own
     float *acc;                               // [row][part][d]
     int *err;
 };
@@ -28,7 +29,34 @@ __device__ __forceinline__ bool prefix_group_fits(int first, int end, int n_seq)
 // positions of sequence s that the shared part covers, were it served there
 __device__ __forceinline__ int prefix_cover(const PrefixArgs &a, int s) { return max(min(a.lens[s], a.shared[s]), 0) / PX_TILE * PX_TILE; }
 
-int launch_prefix_shared(const PrefixArgs &a, int type, cudaStream_t s);   // prefix_attn_tcgen05.cu
-int prefix_shared_rows(int64_t rows);                                      // rows a CTA takes where a (group, key head) has so many
+// prefix_attn_tcgen05.cu: all parts of all rows, in one launch
+int launch_prefix_parts(const PrefixArgs &a, int type, cudaStream_t s);
+constexpr int PX_WARPS = 4, PX_OWN_UNITS = 3;   // warps that share a part of a row's own positions; such parts that a CTA has at work at a time
+int prefix_shared_rows(int64_t rows);      // rows a CTA of the shared part takes where a (group, key head) has so many
+
+#ifdef __CUDACC__
+// The group that sequence s stands in, by a whole warp: its first sequence, or s itself where no group holds it (that is reported).  *served: whether
+// the shared part has computed its whole shared tiles.  A search that looks at 32 places at a time
+__device__ __forceinline__ int prefix_first(const PrefixArgs &a, int s, bool *served) {
+    *served = false;
+    if (a.n_group == 0) return s;
+    const int lane = threadIdx.x & 31;
+    int g = 0, n = a.n_group;
+    while (n > 1) {
+        const int step = (n + 31) / 32, at = lane * step;
+        const bool behind = at < n && a.group_first[g + at] <= s;
+        const int last = 31 - __clz(__ballot_sync(0xffffffffu, behind) | 1u);
+        g += last * step;
+        n = min(step, n - last * step);
+    }
+    const int first = a.group_first[g], end = a.group_first[g + 1];
+    if (!prefix_group_fits(first, end, a.n_seq) || s < first || s >= end) {
+        if (lane == 0) atomicExch(a.err, ERR_PAGED);
+        return s;
+    }
+    *served = s - first < a.served;
+    return first;
+}
+#endif
 
 }  // namespace b200

@@ -13,15 +13,14 @@
 //   * A tile's weights are taken under the maximum in use without a look at its scores; only where their sum exceeds 2^12 (or the row has seen nothing yet) are they taken
 //     again under the tile's own maximum, and the output rescaled: the weights' rounding is relative, so nothing is lost.
 // Every wait is bounded; a wait that runs out raises the CTA's abort flag and the device error word, and its rows are marked so that none is stored.
-#include "attn_tcgen05.cuh"
-#include "prefix_attn.cuh"
+#include "prefix_attn_own.cuh"
 
 namespace b200 {
 
 namespace {
 
 constexpr int TC_M = 128, TC_N = PX_TILE, TC_THREADS = 384, TC_SM_WARP0 = 4, TC_SLOTS_MAX = 8;
-constexpr int TC_REGS = 128, TC_FEW_REGS = 40, TC_MANY_REGS = 168;   // a thread's at launch, then of the loading and of the softmax warps
+constexpr int TC_REGS = 168, TC_FEW_REGS = 56, TC_MANY_REGS = 216;   // a thread's at launch, then of the loading and of the softmax warps
 constexpr int TC_ERR_WAIT = 4;
 constexpr float TC_MOST = 4096.0f;   // sum of a tile's weights up to which the maximum in use is kept
 static_assert(TC_FEW_REGS * TC_SM_WARP0 * 32 + TC_MANY_REGS * (TC_THREADS - TC_SM_WARP0 * 32) <= TC_REGS * TC_THREADS, "register shares");
@@ -30,8 +29,8 @@ template <typename T, int D, bool TWO>
 struct TcCfg {
     static constexpr int CHUNKS = D / 64;               // 64 elements = one 128-byte swizzled box
     static constexpr int TILE = TC_N * D * 2, Q = TC_M * D * 2 * (TWO ? 2 : 1);
-    static constexpr int SLOTS = D == 128 ? (TWO ? 3 : 4) : TC_SLOTS_MAX;
-    static constexpr int SMEM = Q + SLOTS * TILE + 256;   // the barriers behind the operands: nothing is static, so that the operands begin where shared memory does
+    static constexpr int SLOTS = D == 128 ? (TWO ? 4 : 5) : TC_SLOTS_MAX;
+    static constexpr int SHARED = Q + SLOTS * TILE + 256, OWN = PX_OWN_UNITS * (int)sizeof(PxUnit<D>), SMEM = SHARED > OWN ? SHARED : OWN;   // the barriers behind the operands: nothing is static, so that the operands begin where shared memory does
     static constexpr uint32_t O_COL = 2 * TC_N;         // tensor memory: two score tiles, then two outputs
     static constexpr uint32_t TYPES = sizeof(T) == 2 && !std::is_same<T, __half>::value ? (1u << 7) | (1u << 10) : 0u;   // A and B are BF16
     static constexpr uint32_t IDESC_S = (1u << 4) | TYPES | ((uint32_t)(TC_N >> 3) << 17) | ((uint32_t)(TC_M >> 4) << 24);
@@ -79,11 +78,20 @@ __device__ __forceinline__ float2 tc_ex2_pair(uint64_t y) {
 }
 
 template <typename T, int D, bool TWO>
-__global__ void __maxnreg__(TC_REGS)
-prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefixArgs a, const TcArgs ta) {
+__global__ void __launch_bounds__(TC_THREADS, 1)
+prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefixArgs a, const TcArgs ta) {
     using C = TcCfg<T, D, TWO>;
     constexpr int ROWS = TWO ? 2 * TC_M : TC_M;
     extern __shared__ __align__(1024) uint8_t tc_raw[];
+    const int64_t shared_ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts;
+    if (blockIdx.x >= shared_ctas) {
+        static_assert(PX_OWN_UNITS * PX_NT == TC_THREADS && sizeof(PxUnit<D>) % 128 == 0, "units of a CTA");
+        const int unit = threadIdx.x / PX_NT;
+        pdl_wait();
+        pdl_trigger();
+        prefix_own_stream<T, D>(a, (blockIdx.x - shared_ctas) * PX_OWN_UNITS + unit, (int64_t)a.own_ctas * PX_OWN_UNITS, ((PxUnit<D> *)tc_raw)[unit], threadIdx.x % PX_NT, 1 + unit);
+        return;
+    }
     static_assert(sizeof(TcShared) <= 256, "barriers");
     TcShared &sh = *(TcShared *)(tc_raw + C::Q + C::SLOTS * C::TILE);
     const uint32_t q_s = pa_smem(tc_raw), kv_s = q_s + C::Q;
@@ -124,7 +132,7 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
     pa_fence_after();
     const uint32_t tmem = sh.tmem_base;
     pdl_wait();      // q, the cache rows of this step and the lengths come from earlier kernels
-    pdl_trigger();   // whoever starts now may count on these
+    pdl_trigger();
     // the group's rows: row x is sequence first + x / each, head hk * each + x % each
     int first = a.group_first[grp], end = a.group_first[grp + 1];
     const bool fits = prefix_group_fits(first, end, a.n_seq);
@@ -146,7 +154,10 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
 
     if (warp < TC_SM_WARP0) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TC_FEW_REGS));
-        if (warp == 0 && n_tiles > 0) {
+        if ((warp == 0 || warp == 2) && n_tiles > 0) {
+            // warp 0 asks for the keys, warp 2 for the values: a box costs the asking warp some 115 clocks, and a tile of small pages has 16
+            const bool keys = warp == 0;
+            const CUtensorMap *const map = keys ? &kmap : &vmap;
             const int boxes = TC_N / ta.box, my_box = lane % boxes, my_chunk = lane / boxes;   // up to 8 boxes x 2 chunks
             const bool mine = lane < boxes * C::CHUNKS;
             const int32_t *const table = a.cache.tables + (int64_t)first * a.cache.table_ld;
@@ -162,38 +173,26 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
                 }
                 return p;
             };
-            int seq = 0;
+            const int mute = !keys && blockIdx.x == 0 ? ta.mute : -1;
             bool ok = true;
-            const int mute = blockIdx.x == 0 ? ta.mute : -1;
-            auto load = [&](const CUtensorMap *map, int t, int page, bool ask) {
-                const int s = seq % C::SLOTS;
+            int page = page_of(0), t = 0, begun = -1;
+            for (; t < n_tiles; t++) {
+                const int next = page_of(t + 1);
+                // the order in which the products read them: with two blocks K 0, V 0, K 1, .., with one K 0, K 1, V 0, K 2, V 1, ..
+                const int seq = TWO ? 2 * t + !keys : keys ? (t < 2 ? t : 2 * t - 1) : min(2 * t + 2, n_tiles + t), s = seq % C::SLOTS;
                 ok = ok && pa_wait(&sh.empty[s], ((uint32_t)(seq / C::SLOTS) & 1u) ^ 1u, abort_flag, ta.wait_limit);
-                if (!ok) return;
+                if (t == (keys ? 1 : 0)) ok = ok && pa_wait(&sh.qready, 0, abort_flag, ta.wait_limit);   // the queries are needed before these are
+                if (!ok) break;
                 if (lane == 0) pa_expect(&sh.full[s], C::TILE);
                 __syncwarp();
-                if (mine && ask)
+                if (mine && t != mute)
                     tc_tma(kv_s + (uint32_t)(s * C::TILE + my_chunk * (TC_N * 128) + my_box * ta.box * 128), map, 64 * my_chunk, hk, ((t0 + t) * TC_N + my_box * ta.box) & page_mask, page, &sh.full[s]);
-                seq++;
-            };
-            // K 0, (K 1,) then V v and the next K, the order in which the products read them
-            constexpr int AHEAD = TWO ? 1 : 2;
-            int page[AHEAD + 1];
-#pragma unroll
-            for (int i = 0; i <= AHEAD; i++) page[i] = page_of(i);
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++)
-                if (i < n_tiles) load(&kmap, i, page[i], true);
-            for (int v = 0; v < n_tiles && ok; v++) {
-                const int next = page_of(v + AHEAD + 1);
-                load(&vmap, v, page[0], v != mute);
-                if (ok && v + AHEAD < n_tiles) load(&kmap, v + AHEAD, page[AHEAD], true);
-#pragma unroll
-                for (int i = 0; i < AHEAD; i++) page[i] = page[i + 1];
-                page[AHEAD] = next;
+                begun = seq;
+                page = next;
             }
-            // a CTA that gives up still waits (bounded) for the copies it has in flight: a slot's last one
+            // a CTA that gives up still waits (bounded) for the copies it has in flight: those since the slots' last turn
             if (*abort_flag)
-                for (int q = seq > C::SLOTS ? seq - C::SLOTS : 0; q < seq; q++) pa_drain(&sh.full[q % C::SLOTS], (uint32_t)(q / C::SLOTS) & 1u, ta.wait_limit);
+                for (int q = max(begun - C::SLOTS + 1, 0); q <= begun; q++) pa_drain(&sh.full[q % C::SLOTS], (uint32_t)(q / C::SLOTS) & 1u, ta.wait_limit);
         } else if (warp == 1 && n_tiles > 0) {
             // the whole warp waits, one elected lane issues: descriptors then stay in uniform registers
             const bool leader = pa_elect();
@@ -248,7 +247,7 @@ prefix_shared_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_cons
         const int x = (TWO ? g * TC_M : 0) + r;
         const bool live = x < n_rows;
         const int seq = first + (live ? (x0 + x) / a.each : 0), head = hk * a.each + (live ? (x0 + x) % a.each : 0);
-        const int64_t out = ((int64_t)seq * a.n_head + head) * (a.shared_parts + a.own_parts) + part;
+        const int64_t out = ((int64_t)seq * a.n_head + head) * (a.shared_parts + PX_WARPS * a.own_parts) + part;
         const int my_tiles = live ? min(prefix_cover(a, seq) / PX_TILE, n_all) - t0 : 0;   // tiles of this part that the row sees
         if (n_tiles > 0) {
             // q into the swizzled K-major operand, zeros behind the last row: a warp takes ROWS / 8 rows, a lane 16 bytes at a time, all under way at once (row by row
@@ -410,20 +409,22 @@ int launch(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
     B200_REQUIRE(paged_tile_map(&km, type, a.cache.k, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box) &&
                      paged_tile_map(&vm, type, a.cache.v, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box),
                  "prefix_attn: tensor maps over %lld pages of %d positions refused", (long long)a.cache.n_pages, page);
-    B200_CUDA(cudaFuncSetAttribute(prefix_shared_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    B200_CUDA(cudaFuncSetAttribute(prefix_parts_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     // the warps' register shares come out of what the block is launched with
-    cudaFuncAttributes fa;
-    B200_CUDA(cudaFuncGetAttributes(&fa, prefix_shared_kernel<T, D, TWO>));
-    B200_REQUIRE(fa.numRegs >= TC_REGS, "prefix_attn: a build with %d registers a thread cannot share them out", fa.numRegs);
-    const int64_t ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts;
-    return launch_pdl(prefix_shared_kernel<T, D, TWO>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
+    static const int regs = [] {
+        cudaFuncAttributes fa;
+        return cudaFuncGetAttributes(&fa, prefix_parts_kernel<T, D, TWO>) == cudaSuccess ? fa.numRegs : 0;
+    }();
+    B200_REQUIRE(regs >= TC_REGS, "prefix_attn: a build with %d registers a thread cannot share them out", regs);
+    const int64_t ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts + a.own_ctas;
+    return launch_pdl(prefix_parts_kernel<T, D, TWO>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
 }
 
 }  // namespace
 
 int prefix_shared_rows(int64_t rows) { return rows > TC_M ? 2 * TC_M : TC_M; }
 
-int launch_prefix_shared(const PrefixArgs &a, int type, cudaStream_t s) {
+int launch_prefix_parts(const PrefixArgs &a, int type, cudaStream_t s) {
     const bool two = prefix_shared_rows((int64_t)a.served * a.each) == 2 * TC_M;
     if (type == B200_TYPE_F16) {
         if (a.cache.d == 128) return two ? launch<__half, 128, true>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s) : launch<__half, 128, false>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s);
