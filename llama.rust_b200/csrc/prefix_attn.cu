@@ -92,8 +92,9 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
     for (int c = 0; c < C; c++) fine &= fabsf(v[c]) < INFINITY;
     if (!__all_sync(0xffffffffu, fine)) {   // again, position by position
         const T *const q = (const T *)(a.q + (int64_t)s * a.q_nb1 + (int64_t)h * a.q_nb2) + C * lane;
-        bool served;
-        const int first = prefix_first(a, s, &served), shared = a.n_group ? a.shared[s] : 0;
+        int first, end;
+        prefix_group(a, s, &first, &end);
+        const int shared = a.n_group ? a.shared[s] : 0;
         float m = sink;
         L = sink > -INFINITY ? 1.0f : 0.0f;
 #pragma unroll
@@ -138,8 +139,8 @@ struct PrefixPlan {
 
 // Into how many parts the positions are cut, and how the SMs are dealt out between the shared part (a CTA a part, one an SM, first) and the own part
 // (CTAs that walk the items, three at a time): what takes least by a model of the launch.  Times in ns, measured with 8 key heads of 128 and of 64
-// channels: a CTA of the shared part about 8000 and, a tile, 1850 with two blocks of rows, 1400 (an SM takes in 50 GB/s) with one; a unit of the own part 4000, 500
-// an item and 1950 a tile beside two others (the same 50 GB/s); a row's partial output crosses L2 twice at about 5 bytes a picosecond.
+// channels: a CTA of the shared part about 10000 and, a tile, 1850 with two blocks of rows, 5500 and 1300 (an SM takes in 50 GB/s) with one; a unit of the own part 4000, 700
+// an item and, a tile, 650 for each of the SM's units (the same 50 GB/s), at least 1000; a row's partial output crosses L2 twice at about 5 bytes a picosecond.
 struct PartsPlan {
     int64_t d, rows, shared_items, shared_tiles, own_items, own_tiles;
     bool two_blocks;
@@ -148,19 +149,20 @@ struct PartsPlan {
 void plan_parts(PartsPlan *p, int64_t sms) {
     static const int counts[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 18, 24, 32, 48, 64};
     static_assert(PX_MAX_PARTS == 64, "the most parts there are");
-    const int64_t wide = p->d == 128, c_shared = p->two_blocks ? (wide ? 1850 : 1300) : (wide ? 1400 : 800), c_own = wide ? 1950 : 975;
+    const int64_t wide = p->d == 128, c_shared = p->two_blocks ? (wide ? 1850 : 1300) : (wide ? 1300 : 950), f_shared = p->two_blocks ? 10000 : 5500;
     int64_t best = INT64_MAX;
     p->shared_parts = p->own_parts = p->own_ctas = 1;
     if (p->own_items == 0) return;
     for (int ns : counts) {
         if (ns > 1 && ns > p->shared_tiles) break;
-        const int64_t n1 = p->shared_tiles ? p->shared_items * ns : 0, t1 = n1 ? 8000 + c_shared * ((p->shared_tiles + ns - 1) / ns) : 0;
+        const int64_t n1 = p->shared_tiles ? p->shared_items * ns : 0, t1 = n1 ? f_shared + c_shared * ((p->shared_tiles + ns - 1) / ns) : 0;
         const int64_t waves = n1 / sms, left = sms - (n1 - waves * sms);   // SMs that the last wave leaves
         if (ns > 1 && n1 > 2 * sms) break;
         for (int no : counts) {
             if (no > 1 && no > p->own_tiles) break;
-            const int64_t items = p->own_items * no, units = (items + PX_OWN_UNITS - 1) / PX_OWN_UNITS, ctas = units < left ? units : left;
-            const int64_t each = (items + ctas * PX_OWN_UNITS - 1) / (ctas * PX_OWN_UNITS), t2 = 4000 + each * (500 + c_own * ((p->own_tiles + no - 1) / no));
+            const int64_t items = p->own_items * no, ctas = items < left ? items : left, units = items < 3 * ctas ? (items + ctas - 1) / ctas : 3;
+            const int64_t each = (items + ctas * units - 1) / (ctas * units), tile = (wide ? 650 : 325) * units > 1000 ? (wide ? 650 : 325) * units : 1000;
+            const int64_t t2 = 4000 + each * (700 + tile * ((p->own_tiles + no - 1) / no));
             const int64_t shared = (waves + (n1 > waves * sms)) * t1, own = waves * t1 + t2;
             const int64_t time = (shared > own ? shared : own) + p->rows * (PX_WARPS * no + (n1 ? ns : 0)) * p->d * 8 / 5000;
             if (time < best) {
@@ -212,7 +214,7 @@ int prefix_plan(const b200_prefix_attn_args &g, PrefixPlan *p) {
     a.shared_parts = a.served ? pp.shared_parts : 0;
     a.own_parts = pp.own_parts;
     a.own_ctas = pp.own_ctas;
-    B200_REQUIRE(pp.shared_items < (1 << 24) && pp.own_items < (1 << 24), "prefix_attn: too many rows for one launch");
+    B200_REQUIRE(pp.shared_items < (1 << 24) && pp.own_items < (1 << 23), "prefix_attn: too many rows for one launch");
     const int64_t slots = p->rows * (a.shared_parts + PX_WARPS * a.own_parts);
     p->ml_bytes = ((size_t)slots * sizeof(float2) + 255) & ~(size_t)255;
     p->bytes = p->ml_bytes + (size_t)slots * (size_t)g.cache.d * 4;

@@ -35,11 +35,12 @@ constexpr int PX_WARPS = 4, PX_OWN_UNITS = 3;   // warps that share a part of a 
 int prefix_shared_rows(int64_t rows);      // rows a CTA of the shared part takes where a (group, key head) has so many
 
 #ifdef __CUDACC__
-// The group that sequence s stands in, by a whole warp: its first sequence, or s itself where no group holds it (that is reported).  *served: whether
-// the shared part has computed its whole shared tiles.  A search that looks at 32 places at a time
-__device__ __forceinline__ int prefix_first(const PrefixArgs &a, int s, bool *served) {
-    *served = false;
-    if (a.n_group == 0) return s;
+// The group that sequence s stands in, by a whole warp: its first sequence and the one behind its last; s alone where nothing is shared, and where no group holds it
+// (that is reported: false).  A search that looks at 32 places at a time
+__device__ __forceinline__ bool prefix_group(const PrefixArgs &a, int s, int *first, int *end) {
+    *first = s;
+    *end = s + 1;
+    if (a.n_group == 0) return false;
     const int lane = threadIdx.x & 31;
     int g = 0, n = a.n_group;
     while (n > 1) {
@@ -49,13 +50,14 @@ __device__ __forceinline__ int prefix_first(const PrefixArgs &a, int s, bool *se
         g += last * step;
         n = min(step, n - last * step);
     }
-    const int first = a.group_first[g], end = a.group_first[g + 1];
-    if (!prefix_group_fits(first, end, a.n_seq) || s < first || s >= end) {
+    const int f = a.group_first[g], e = a.group_first[g + 1];
+    if (!prefix_group_fits(f, e, a.n_seq) || s < f || s >= e) {
         if (lane == 0) atomicExch(a.err, ERR_PAGED);
-        return s;
+        return false;
     }
-    *served = s - first < a.served;
-    return first;
+    *first = f;
+    *end = e;
+    return true;
 }
 #endif
 

@@ -66,12 +66,12 @@ struct alignas(128) PxUnit {                  // shared memory of four warps
 // every tile, its own maximum and sum, and leaves a part of its own for the merge.  Positions that the sequence does not see are zeros in shared memory,
 // whatever the page holds.  tid: 0 .. 127; barrier: a named one of these four warps
 template <typename T, int D>
-__device__ __forceinline__ void prefix_own_stream(const PrefixArgs &a, int64_t unit, int64_t n_units, PxUnit<D> &sh, int tid, int barrier) {
+__device__ __forceinline__ void prefix_own_stream(const PrefixArgs &a, int unit, int n_units, PxUnit<D> &sh, int tid, int barrier) {
     constexpr int KS = D / 16, DB = D / 8, NST = PX_STAGES<D>;
     constexpr int PIECES = D / 8, RSTEP = PX_NT / PIECES, PASSES = PX_BN / RSTEP;   // a thread's pieces of a tile: 16 bytes tid % PIECES of rows tid / PIECES + RSTEP j
     static_assert(RSTEP % 8 == 0, "a thread's rows have one place for their piece");
     const int lane = tid & 31, warp = tid >> 5;
-    const int64_t n_items = (int64_t)a.n_seq * a.cache.n_head_kv * a.own_blocks * a.own_parts;
+    const int n_items = a.n_seq * a.cache.n_head_kv * a.own_blocks * a.own_parts, of_seq = a.cache.n_head_kv * a.own_blocks * a.own_parts;   // below 2^30
     const int all_parts = a.shared_parts + PX_WARPS * a.own_parts;
     const int capacity = (int)(a.cache.table_ld < (0x7fffff00 >> a.cache.page_log2) ? a.cache.table_ld << a.cache.page_log2 : 0x7fffff00);
     auto sync = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(PX_NT) : "memory"); };
@@ -79,26 +79,35 @@ __device__ __forceinline__ void prefix_own_stream(const PrefixArgs &a, int64_t u
     // ---- the loading side: item `next_item`'s tile `tile` comes next
     PxItem it;
     it.n = 0;
-    int64_t next_item = unit - n_units;
+    int next_item = unit - n_units;
     int tile = 0, tasks = 0;   // tasks: items handed to the multiplying side so far
+    // an item's length and shared positions are read an item ahead
+    int ahead_len = 0, ahead_shared = 0, grp_first = 0, grp_end = 0;   // the group of the item before: most likely this one's too
+    bool in_group = false;
+    auto read_ahead = [&](int item) {
+        if (item < n_items) {
+            ahead_len = a.lens[item / of_seq];
+            ahead_shared = a.n_group ? a.shared[item / of_seq] : 0;
+        }
+    };
+    read_ahead(unit);
     // on to the next item with tiles; false: there is none
     auto advance = [&]() -> bool {
         while (tile >= it.n) {
-            next_item += n_units;
-            if (next_item >= n_items) {
-                next_item = n_items;
-                return false;
-            }
-            int64_t id = next_item;
-            it.part = (int)(id % a.own_parts); id /= a.own_parts;
-            it.x0 = (int)(id % a.own_blocks) * PX_BM; id /= a.own_blocks;
-            it.hk = (int)(id % a.cache.n_head_kv);
-            it.s = (int)(id / a.cache.n_head_kv);
+            next_item = min(next_item + n_units, n_items);
+            if (next_item == n_items) return false;
+            it.s = next_item / of_seq;
+            int id = next_item - it.s * of_seq;
+            it.part = id % a.own_parts; id /= a.own_parts;
+            it.x0 = id % a.own_blocks * PX_BM;
+            it.hk = id / a.own_blocks;
             it.rows = min(a.each - it.x0, PX_BM);
-            const int len = a.lens[it.s];
-            it.shared = a.n_group ? a.shared[it.s] : 0;
-            bool served;
-            it.first = prefix_first(a, it.s, &served);
+            const int len = ahead_len;
+            it.shared = ahead_shared;
+            read_ahead(next_item + n_units);
+            if (it.s < grp_first || it.s >= grp_end) in_group = prefix_group(a, it.s, &grp_first, &grp_end);
+            it.first = grp_first;
+            const bool served = in_group && it.s - grp_first < a.served;
             if (len > capacity && tid == 0) atomicExch(a.err, ERR_PAGED);
             it.end = min(len, capacity);
             const int lo = served ? min(max(min(len, it.shared), 0), capacity) / PX_TILE * PX_TILE : 0;

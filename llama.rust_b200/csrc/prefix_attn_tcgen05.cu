@@ -89,7 +89,7 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         const int unit = threadIdx.x / PX_NT;
         pdl_wait();
         pdl_trigger();
-        prefix_own_stream<T, D>(a, (blockIdx.x - shared_ctas) * PX_OWN_UNITS + unit, (int64_t)a.own_ctas * PX_OWN_UNITS, ((PxUnit<D> *)tc_raw)[unit], threadIdx.x % PX_NT, 1 + unit);
+        prefix_own_stream<T, D>(a, (int)(blockIdx.x - shared_ctas) + unit * a.own_ctas, a.own_ctas * PX_OWN_UNITS, ((PxUnit<D> *)tc_raw)[unit], threadIdx.x % PX_NT, 1 + unit);
         return;
     }
     static_assert(sizeof(TcShared) <= 256, "barriers");
