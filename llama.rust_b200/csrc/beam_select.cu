@@ -22,9 +22,9 @@ namespace {
 
 constexpr int BS_NT = 256, BS_MAX_K = 128, BS_MAX_BEAM = 64;
 constexpr int BS_LIST = 512;            // candidates that are ordered by counting
-constexpr int BS_MERGE_NT = 512, BS_CACHE = 4096;   // 32 KB of scores
+constexpr int BS_MERGE_NT = 512, BS_HELD = 4;   // threads of the merge; candidates each keeps in registers
 
-struct Cand {                            // of a chunk, in descending order
+struct Cand {                            // of a chunk, in descending order; behind its last one -inf
     float value;
     int token;
 };
@@ -35,7 +35,6 @@ struct SelectArgs {
     int64_t ld, n_vocab;
     int n_beam, k, chunks, end_token;
     Cand *cand;                          // [row][chunk][k]
-    int *count;                          // [row][chunk]
     float *top;                          // [row][chunk]
     double *sum;                         // [row][chunk]
     float *out_scores;
@@ -51,6 +50,18 @@ __device__ __forceinline__ uint64_t order64(double x) {
     const uint64_t b = (uint64_t)__double_as_longlong(x + 0.0);
     return b >> 63 ? ~b : b | (1ull << 63);
 }
+__device__ __forceinline__ float value32(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+constexpr float LOG2E = 1.4426950408889634f, LOWEST = -3.402823466e38f;   // the least finite value
 constexpr uint32_t ORDER32_NONE = 0x007fffffu;               // of -inf
 constexpr uint64_t ORDER64_NONE = 0x000fffffffffffffull;
 
@@ -124,7 +135,7 @@ template <typename T, int EPT>
 __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
     constexpr int N = Unpack<T>::N, VECS = EPT / N;
     pdl_trigger();
-    __shared__ float warp_top[BS_NT / 32];
+    __shared__ __align__(16) float group_top[32];
     __shared__ double warp_sum[BS_NT / 32];
     __shared__ uint64_t list[BS_LIST];       // order of the value, then the complement of the token: larger is better
     __shared__ int n_list, part[BS_NT / 32];
@@ -136,67 +147,107 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
     const uint8_t *const base = a.logits + row * a.ld * (int64_t)sizeof(T), *const row_end = base + a.n_vocab * (int64_t)sizeof(T);
     const int first = chunk * BS_NT * EPT;   // the vocabulary is below 2^31
     float x[EPT];
+    if ((int64_t)first + BS_NT * EPT <= a.n_vocab && ((uintptr_t)base & 15) == 0) {
+        uint4 w[VECS];
 #pragma unroll
-    for (int v = 0; v < VECS; v++) {
-        const int64_t e = (int64_t)first + (int64_t)(v * BS_NT + tid) * N;
-        if (e < a.n_vocab) {
-            uint32_t w[4];
-            load16<T>(base + e * (int64_t)sizeof(T), row_end, base, row_end, w);
-            Unpack<T>::get(w, x + v * N);
-        } else {
+        for (int v = 0; v < VECS; v++) w[v] = ld_stream16(base + (first + (v * BS_NT + tid) * N) * (int64_t)sizeof(T));
 #pragma unroll
-            for (int i = 0; i < N; i++) x[v * N + i] = -INFINITY;
+        for (int v = 0; v < VECS; v++) {
+            const uint32_t u[4] = {w[v].x, w[v].y, w[v].z, w[v].w};
+            Unpack<T>::get(u, x + v * N);
+        }
+    } else {   // the row's end, and rows that begin anywhere
+#pragma unroll
+        for (int v = 0; v < VECS; v++) {
+            const int64_t e = (int64_t)first + (int64_t)(v * BS_NT + tid) * N;
+            if (e < a.n_vocab) {
+                uint32_t w[4];
+                load16<T>(base + e * (int64_t)sizeof(T), row_end, base, row_end, w);
+                Unpack<T>::get(w, x + v * N);
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; i++) x[v * N + i] = -INFINITY;
+            }
         }
     }
     float mine = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        if (x[i] != x[i]) x[i] = -INFINITY;
-        mine = fmaxf(mine, x[i]);
+    for (int i = 0; i < EPT; i += 2) {
+        x[i] = fmaxf(x[i], -INFINITY);   // a NaN counts as -inf
+        x[i + 1] = fmaxf(x[i + 1], -INFINITY);
+        mine = max3(mine, x[i], x[i + 1]);
     }
-    float m = mine;
+    // maxima of groups of 8 threads, then of the chunk
+    float g = mine;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((tid & 31) == 0) warp_top[tid >> 5] = m;
+    for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if ((tid & 7) == 0) group_top[tid >> 3] = g;
     if (tid == 0) n_list = 0;
     __syncthreads();
+    const int lane = tid & 31;
+    const float mine_g = group_top[lane];
+    float m = mine_g;
 #pragma unroll
-    for (int i = 0; i < BS_NT / 32; i++) m = fmaxf(m, warp_top[i]);
-    // sum of exponentials
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // sum of exponentials: exp2(x log2(e) - c) with c = m log2(e) rounded, one multiply-add each; what the rounding of c is off by, the merge puts right
     float s = 0.0f;
-    if (m > -INFINITY) {
+    if (fabsf(m) < 1e30f) {
+        const float c = m * LOG2E;
+        float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < EPT; i++) s += x[i] == m ? 1.0f : exp2f((x[i] - m) * 1.4426950408889634f);
+        for (int i = 0; i < EPT; i++) s4[i & 3] += fast_exp2(fmaf(x[i], LOG2E, -c));
+        s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    } else if (m > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < EPT; i++) s += x[i] == m ? 1.0f : exp2f((x[i] - m) * LOG2E);
     }
     double ds = (double)s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
-    if ((tid & 31) == 0) warp_sum[tid >> 5] = ds;
-    // a bound that k values of the chunk reach: bisected until few more threads than that have one (then the list has room for what
-    // independent values put above it: at 192 of 256 threads about 355)
-    uint32_t lo = ORDER32_NONE + 1, hi = order32(m);   // k values reach lo, or lo lets every finite value pass
-    const uint32_t best = order32(mine);
-    const int enough = 2 * a.k < 192 ? 2 * a.k : 192;
-    uint32_t top = hi;
-    if (block_count(best >= lo) > enough) {
-        while (lo < top) {
-            const uint32_t at = lo + (top - lo + 1) / 2;
-            const int c = block_count(best >= at);
-            if (c >= a.k) {
-                lo = at;
-                if (c <= enough) break;
-            } else {
-                top = at - 1;
-            }
-        }
-    }
-    int n = 0;
+    if (lane == 0) warp_sum[tid >> 5] = ds;
+    // A bound that k values of the chunk reach and few more do.  Up to 32 candidates: the k-th largest of the 32 groups' maxima, which every warp ranks for
+    // itself (independent values: 22 above it with k = 16, 130 with 32).  More: bisected over the threads' maxima until few more than k of the 256 have one
+    // (at 192 about 355 values).  It lets every finite value pass where fewer than k maxima are finite
+    float bound;
+    if (a.k <= 32) {
+        int better = 0;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) n += order32(x[i]) >= lo;
-    n = block_total(n, part);
-    int last = 0x7fffffff;       // of the values that equal the bound only those up to this token
-    if (n > BS_LIST) {           // the k-th largest value itself
-        top = hi;
+        for (int j = 0; j < 32; j += 4) {
+            const float4 o = *(const float4 *)(group_top + j);
+            better += (o.x > mine_g || (o.x == mine_g && j < lane)) + (o.y > mine_g || (o.y == mine_g && j + 1 < lane)) + (o.z > mine_g || (o.z == mine_g && j + 2 < lane)) +
+                      (o.w > mine_g || (o.w == mine_g && j + 3 < lane));
+        }
+        bound = __shfl_sync(0xffffffffu, mine_g, __ffs(__ballot_sync(0xffffffffu, better == a.k - 1)) - 1);
+    } else {
+        uint32_t lo = ORDER32_NONE + 1, top = order32(m);
+        const uint32_t best = order32(mine);
+        const int enough = 2 * a.k < 192 ? 2 * a.k : 192;
+        if (block_count(best >= lo) > enough)
+            while (lo < top) {
+                const uint32_t at = lo + (top - lo + 1) / 2;
+                const int c = block_count(best >= at);
+                if (c >= a.k) {
+                    lo = at;
+                    if (c <= enough) break;
+                } else {
+                    top = at - 1;
+                }
+            }
+        bound = value32(lo);
+    }
+    bound = fmaxf(bound, LOWEST);
+    if (mine >= bound) {
+#pragma unroll
+        for (int i = 0; i < EPT; i++)
+            if (x[i] >= bound) {
+                const int at = atomicAdd(&n_list, 1);
+                if (at < BS_LIST) list[at] = (uint64_t)order32(x[i]) << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
+            }
+    }
+    __syncthreads();
+    int n = n_list;
+    if (n > BS_LIST) {           // too many reach it: the k-th largest value itself, and of its equals the first
+        uint32_t lo = order32(bound), top = order32(m);
         while (lo < top) {
             const uint32_t at = lo + (top - lo + 1) / 2;
             int c = 0;
@@ -218,31 +269,26 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
             if (block_total(c, part) >= want) h = at;
             else l = at + 1;
         }
-        last = l;
-    }
+        if (tid == 0) n_list = 0;
+        __syncthreads();
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {
-        const uint32_t o = order32(x[i]);
-        if (o > lo || (o == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= last)) {
-            const int at = atomicAdd(&n_list, 1);
-            if (at < BS_LIST) list[at] = (uint64_t)o << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
+        for (int i = 0; i < EPT; i++) {
+            const uint32_t o = order32(x[i]);
+            if (o > lo || (o == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= l)) list[atomicAdd(&n_list, 1)] = (uint64_t)o << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
         }
+        __syncthreads();
+        n = n_list;
     }
-    __syncthreads();
-    n = n_list < BS_LIST ? n_list : BS_LIST;
     Cand *const out = a.cand + slot * a.k;
     for (int i = tid; i < n; i += BS_NT) {
         const uint64_t me = list[i];
         int better = 0;
+#pragma unroll 8
         for (int j = 0; j < n; j++) better += list[j] > me;
-        if (better < a.k) {
-            const uint32_t o = (uint32_t)(me >> 32);
-            out[better].value = __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
-            out[better].token = (int)~(uint32_t)me;
-        }
+        if (better < a.k) out[better] = {value32((uint32_t)(me >> 32)), (int)~(uint32_t)me};
     }
-    if (tid == 0) {
-        a.count[slot] = n < a.k ? n : a.k;
+    for (int i = n + tid; i < a.k; i += BS_NT) out[i] = {-INFINITY, 0};
+    if (tid == BS_NT - 1) {
         a.top[slot] = m;
         double t = 0.0;
 #pragma unroll
@@ -251,143 +297,163 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
     }
 }
 
-__global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArgs a, int n_cached) {
+// One candidate of a request: its place among them (beam, chunk, place in the chunk's list) gives the beam
+struct MergeView {
+    const double *offset;
+    const float *top;
+    int per_beam;
+    __device__ __forceinline__ uint64_t order(int i, float value) const {
+        const int b = i / per_beam;
+        const float m = top[b];
+        const double off = offset[b];
+        if (off == -INFINITY) return ORDER64_NONE;
+        if (m != m) return i == b * per_beam ? order64(off) : ORDER64_NONE;   // an ended beam's only one
+        return order64(value == m ? off : off + ((double)value - (double)m));
+    }
+};
+
+__global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArgs a) {
     pdl_trigger();
-    extern __shared__ uint64_t cached[];     // scores of the first n_cached candidates
     __shared__ double offset[BS_MAX_BEAM];   // score of a beam less the logarithm of its sum
     __shared__ float top_s[BS_MAX_BEAM];
     __shared__ uint64_t key[BS_LIST];
     __shared__ int64_t where[BS_LIST];       // beam * vocabulary + token
+    __shared__ uint64_t bound_s, best_s;
     __shared__ int n_list, part[BS_MERGE_NT / 32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t r = blockIdx.x, row0 = r * a.n_beam;
+    const int per_beam = a.chunks * a.k, total = a.n_beam * per_beam;
+    const Cand *const cand = a.cand + row0 * per_beam;
     if (tid == 0) n_list = 0;
     pdl_wait();
+    // the first candidates are on their way while the beams' sums are joined
+    Cand mine[BS_HELD];
+#pragma unroll
+    for (int u = 0; u < BS_HELD; u++) mine[u] = tid + u * BS_MERGE_NT < total ? cand[tid + u * BS_MERGE_NT] : Cand{-INFINITY, 0};
     for (int b = warp; b < a.n_beam; b += BS_MERGE_NT / 32) {
         const int64_t row = row0 + b;
         const float score = a.scores[row];
-        const bool off = !(score > -INFINITY);   // -inf or NaN
-        if (a.done && a.done[row]) {
-            if (lane == 0) {
-                offset[b] = off ? -INFINITY : (double)score;
-                top_s[b] = NAN;                  // marks an ended beam
-            }
-            continue;
-        }
+        const bool off = !(score > -INFINITY), ended = a.done && a.done[row];   // off: -inf or NaN
         float m = -INFINITY;
-        for (int c = lane; c < a.chunks; c += 32) m = fmaxf(m, a.top[row * a.chunks + c]);
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         double s = 0.0;
-        for (int c = lane; c < a.chunks; c += 32) {
-            const float t = a.top[row * a.chunks + c];
-            if (t > -INFINITY) s += a.sum[row * a.chunks + c] * (t == m ? 1.0 : exp((double)t - (double)m));
-        }
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (lane == 0) {
-            offset[b] = off || m == -INFINITY ? -INFINITY : (double)score - log(s);
-            top_s[b] = m;
-        }
-    }
-    __syncthreads();
-    // candidate i of the request: beam, chunk, place in the chunk's list
-    const int per_beam = a.chunks * a.k, total = a.n_beam * per_beam;
-    auto order = [&](int i, int64_t *at) -> uint64_t {
-        const int b = i / per_beam, j = i - b * per_beam, c = j / a.k, p = j - c * a.k;
-        const float m = top_s[b];
-        const double off = offset[b];
-        if (off == -INFINITY) return ORDER64_NONE;
-        if (m != m) {
-            *at = (int64_t)b * a.n_vocab + a.end_token;
-            return j == 0 ? order64(off) : ORDER64_NONE;
-        }
-        const int64_t slot = (row0 + b) * a.chunks + c;
-        if (p >= a.count[slot]) return ORDER64_NONE;
-        const Cand cd = a.cand[slot * a.k + p];
-        *at = (int64_t)b * a.n_vocab + cd.token;
-        if (cd.value == m) return order64(off);
-        return order64(off + ((double)cd.value - (double)m));
-    };
-    // bound: k candidates reach lo.  The scores stand in shared memory where there is room for them
-    uint64_t lo = ~0ull, hi = ORDER64_NONE;
-    int64_t at = 0;
-    int n = 0;
-    for (int i = tid; i < total; i += BS_MERGE_NT) {
-        const uint64_t o = order(i, &at);
-        if (i < n_cached) cached[i] = o;
-        if (o == ORDER64_NONE) continue;
-        hi = o > hi ? o : hi;
-        lo = o < lo ? o : lo;
-        n++;
-    }
-    auto again = [&](int i) -> uint64_t { return i < n_cached ? cached[i] : order(i, &at); };   // a thread's own candidates only
+        if (!ended) {
+            float t = lane < a.chunks ? a.top[row * a.chunks + lane] : -INFINITY;
+            double part_sum = lane < a.chunks ? a.sum[row * a.chunks + lane] : 0.0;
+            m = t;
+            for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, a.top[row * a.chunks + c]);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t v = __shfl_xor_sync(0xffffffffu, hi, o), u = __shfl_xor_sync(0xffffffffu, lo, o);
-        hi = v > hi ? v : hi;
-        lo = u < lo ? u : lo;
-    }
-    if (lane == 0) {
-        key[warp] = hi;
-        key[BS_MERGE_NT / 32 + warp] = lo;
-    }
-    n = block_total(n, part);
-    for (int i = 0; i < BS_MERGE_NT / 32; i++) {
-        hi = key[i] > hi ? key[i] : hi;
-        lo = key[BS_MERGE_NT / 32 + i] < lo ? key[BS_MERGE_NT / 32 + i] : lo;
-    }
-    __syncthreads();
-    uint64_t up = hi;
-    int64_t last = 0x7fffffffffffffffLL;
-    const int enough = 2 * a.k > 64 ? 2 * a.k : 64;
-    while (n > enough && lo < up) {
-        const uint64_t mid = lo + (up - lo) / 2 + ((up - lo) & 1);
-        int c = 0;
-        for (int i = tid; i < total; i += BS_MERGE_NT) c += again(i) >= mid;
-        c = block_total(c, part);
-        if (c >= a.k) {
-            lo = mid;
-            n = c;
-        } else {
-            up = mid - 1;
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            for (int c = lane;;) {
+                // exp(t - m), and 2^-(t log2(e) - its rounding) for the chunk's sum
+                if (t > -INFINITY) s += part_sum * (fabsf(t) < 1e30f ? (double)fast_exp2(t == m ? -fmaf(t, LOG2E, -(t * LOG2E)) : (t - m) * LOG2E - fmaf(t, LOG2E, -(t * LOG2E))) : t == m ? 1.0 : exp((double)t - (double)m));
+                c += 32;
+                if (c >= a.chunks) break;
+                t = a.top[row * a.chunks + c];
+                part_sum = a.sum[row * a.chunks + c];
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        }
+        if (lane == 0) {
+            offset[b] = off || (!ended && m == -INFINITY) ? -INFINITY : ended ? (double)score : (double)score - log(s);
+            top_s[b] = ended ? NAN : m;
         }
     }
-    if (n > BS_LIST) {   // more candidates than that have the k-th score: the first by beam and token
-        int above = 0;
-        for (int i = tid; i < total; i += BS_MERGE_NT) above += again(i) > lo;
-        const int want = a.k - block_total(above, part);
+    __syncthreads();
+    const MergeView view = {offset, top_s, per_beam};
+    uint64_t held[BS_HELD], most = ORDER64_NONE;
+#pragma unroll
+    for (int u = 0; u < BS_HELD; u++) {
+        const int i = tid + u * BS_MERGE_NT;
+        held[u] = i < total ? view.order(i, mine[u].value) : ORDER64_NONE;
+        most = held[u] > most ? held[u] : most;
+    }
+    for (int i = tid + BS_HELD * BS_MERGE_NT; i < total; i += BS_MERGE_NT) {
+        const uint64_t o = view.order(i, cand[i].value);
+        most = o > most ? o : most;
+    }
+    // count of a thread's own candidates for which f(order, place) holds
+    auto count = [&](auto f) -> int {
+        int c = 0;
+#pragma unroll
+        for (int u = 0; u < BS_HELD; u++) c += held[u] > ORDER64_NONE && f(held[u], mine[u].token, tid + u * BS_MERGE_NT);
+        for (int i = tid + BS_HELD * BS_MERGE_NT; i < total; i += BS_MERGE_NT) {
+            const Cand cd = cand[i];
+            const uint64_t o = view.order(i, cd.value);
+            c += o > ORDER64_NONE && f(o, cd.token, i);
+        }
+        return c;
+    };
+    auto place = [&](int token, int i) -> int64_t {
+        const int b = i / per_beam;
+        return b * a.n_vocab + (top_s[b] != top_s[b] ? a.end_token : token);
+    };
+    // Bound: k candidates reach lo.  The k-th largest of the maxima of 32 groups of 16 threads (128 of 4, for k > 32) is one that few more reach; fewer than k groups
+    // have any: every candidate passes
+    const int groups = a.k <= 32 ? 32 : 128, width = BS_MERGE_NT / groups;
+    for (int o = width / 2; o > 0; o >>= 1) {
+        const uint64_t v = __shfl_xor_sync(0xffffffffu, most, o);
+        most = v > most ? v : most;
+    }
+    if (tid % width == 0) key[tid / width] = most;
+    __syncthreads();
+    if (tid < groups) {
+        const uint64_t me = key[tid];
+        int better = 0;
+#pragma unroll 8
+        for (int j = 0; j < groups; j++) {
+            const uint64_t other = key[j];
+            better += other > me || (other == me && j < tid);
+        }
+        if (better == a.k - 1) bound_s = me;
+        if (better == 0) best_s = me;
+    }
+    __syncthreads();
+    uint64_t lo = bound_s > ORDER64_NONE ? bound_s : ORDER64_NONE + 1;
+    auto list = [&](uint64_t o, int token, int i) {
+        const int e = atomicAdd(&n_list, 1);
+        if (e < BS_LIST) {
+            key[e] = o;
+            where[e] = place(token, i);
+        }
+        return true;
+    };
+    count([&](uint64_t o, int token, int i) { return o >= lo && list(o, token, i); });
+    __syncthreads();
+    int n = n_list;
+    if (n > BS_LIST) {   // too many reach it: the k-th score itself, and of its equals the first by beam and token
+        uint64_t up = best_s;
+        while (lo < up) {
+            const uint64_t mid = lo + (up - lo) / 2 + ((up - lo) & 1);
+            if (block_total(count([&](uint64_t o, int, int) { return o >= mid; }), part) >= a.k) lo = mid;
+            else up = mid - 1;
+        }
+        const int want = a.k - block_total(count([&](uint64_t o, int, int) { return o > lo; }), part);
         int64_t l = 0, h = a.n_beam * a.n_vocab - 1;
         while (l < h) {
             const int64_t mid = l + (h - l) / 2;
-            int c = 0;
-            for (int i = tid; i < total; i += BS_MERGE_NT) c += order(i, &at) == lo && at <= mid;
-            if (block_total(c, part) >= want) h = mid;
+            if (block_total(count([&](uint64_t o, int token, int i) { return o == lo && place(token, i) <= mid; }), part) >= want) h = mid;
             else l = mid + 1;
         }
-        last = l;
+        if (tid == 0) n_list = 0;
+        __syncthreads();
+        count([&](uint64_t o, int token, int i) { return (o > lo || (o == lo && place(token, i) <= l)) && list(o, token, i); });
+        __syncthreads();
+        n = n_list;
     }
-    for (int i = tid; i < total; i += BS_MERGE_NT) {
-        const uint64_t o = order(i, &at);
-        if (o > lo || (o == lo && at <= last)) {
-            const int e = atomicAdd(&n_list, 1);
-            if (e < BS_LIST) {
-                key[e] = o;
-                where[e] = at;
-            }
-        }
-    }
-    __syncthreads();
-    n = n_list < BS_LIST ? n_list : BS_LIST;
     for (int i = tid; i < n; i += BS_MERGE_NT) {
         const uint64_t me = key[i];
-        const int64_t mine = where[i];
+        const int64_t at = where[i];
         int better = 0;
-        for (int j = 0; j < n; j++) better += key[j] > me || (key[j] == me && where[j] < mine);
+#pragma unroll 8
+        for (int j = 0; j < n; j++) better += key[j] > me || (key[j] == me && where[j] < at);
         if (better < a.k) {
             const int64_t e = r * a.k + better;
             const uint64_t bits = me >> 63 ? me & ~(1ull << 63) : ~me;
+            const int b = (int)(at / a.n_vocab);
             a.out_scores[e] = (float)__longlong_as_double((long long)bits);
-            a.out_parents[e] = (int32_t)(mine / a.n_vocab);
-            a.out_tokens[e] = (int32_t)(mine % a.n_vocab);
+            a.out_parents[e] = b;
+            a.out_tokens[e] = (int32_t)(at - b * a.n_vocab);
         }
     }
     for (int i = n + tid; i < a.k; i += BS_MERGE_NT) {
@@ -408,7 +474,7 @@ int select_ept(int64_t rows, int64_t n_vocab) {
 struct SelectPlan {
     int ept;
     int64_t rows, chunks;
-    size_t cand, count, top, sum, bytes;     // offsets in the workspace
+    size_t cand, top, sum, bytes;     // offsets in the workspace
 };
 size_t up256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -424,8 +490,7 @@ int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
     B200_REQUIRE(p->chunks * g.k * g.n_beam < 0x7fffffffLL, "beam_select: too many candidates of a request");
     const size_t slots = (size_t)(p->rows * p->chunks);
     p->cand = 0;
-    p->count = p->cand + up256(slots * g.k * sizeof(Cand));
-    p->top = p->count + up256(slots * 4);
+    p->top = p->cand + up256(slots * g.k * sizeof(Cand));
     p->sum = p->top + up256(slots * 4);
     p->bytes = p->sum + up256(slots * 8);
     return B200_STATUS_SUCCESS;
@@ -481,7 +546,6 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
     a.chunks = (int)p.chunks;
     a.end_token = g.end_token;
     a.cand = (Cand *)(ws + p.cand);
-    a.count = (int *)(ws + p.count);
     a.top = (float *)(ws + p.top);
     a.sum = (double *)(ws + p.sum);
     a.out_scores = g.out_scores;
@@ -492,9 +556,7 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
     else if (g.logits_type == B200_TYPE_F16) rc = launch_rows<__half>(a, p, s);
     else rc = launch_rows<__nv_bfloat16>(a, p, s);
     if (rc != B200_STATUS_SUCCESS) return rc;
-    const int64_t total = p.chunks * g.n_beam * g.k;
-    const int n_cached = (int)(total < BS_CACHE ? total : BS_CACHE);
-    return launch_pdl(beam_merge_kernel, dim3((unsigned)g.n_request), dim3(BS_MERGE_NT), (size_t)n_cached * 8, s, a, n_cached);
+    return launch_pdl(beam_merge_kernel, dim3((unsigned)g.n_request), dim3(BS_MERGE_NT), 0, s, a);
 }
 
 }  // extern "C"
