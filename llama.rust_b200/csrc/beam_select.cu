@@ -4,7 +4,7 @@
 //   score(b, w) = scores[b] + ((x_w - m) - log sum_v exp(x_v - m)),   m = max_v x_v        (m = +inf: x_w - m is 0 where x_w = m, -inf elsewhere)
 //
 // Bound by reading the logits once.  Two launches:
-//   * beam_rows_kernel: a CTA holds a chunk of a row in registers (256 threads x EPT values), so that maximum, sum of exponentials and the chunk's k best come of
+//   * beam_rows_kernel: a CTA holds a chunk of a row in registers (512 threads x EPT values), so that maximum, sum of exponentials and the chunk's k best come of
 //     one read.  The k best: the k-th largest of the threads' own maxima is a bound that at least k values reach and few more do; a bisection
 //     over counts (one barrier each) comes near enough to it, the values above are listed and ordered by counting the better ones of each.
 //     Where too many reach the bound (equal values), the bisection goes on over all values, then over the indexes of the equal ones.
@@ -20,7 +20,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int BS_NT = 256, BS_MAX_K = 128, BS_MAX_BEAM = 64;
+constexpr int BS_NT = 512, BS_MAX_K = 128, BS_MAX_BEAM = 64;
 constexpr int BS_LIST = 512;            // candidates that are ordered by counting
 constexpr int BS_MERGE_NT = 512, BS_HELD = 4;   // threads of the merge; candidates each keeps in registers
 
@@ -29,7 +29,7 @@ struct Cand {                            // of a chunk, in descending order; beh
     int token;
 };
 struct SelectArgs {
-    const uint8_t *logits;
+    const uint8_t *logits, *logits_end;
     const float *scores;
     const uint8_t *done;
     int64_t ld, n_vocab;
@@ -76,6 +76,16 @@ __device__ __forceinline__ int block_total(int v, int *part) {   // sum over the
     return t;
 }
 
+// the 16 bytes `shift` bytes into two neighbouring vectors; shift is the same for a whole row
+__device__ __forceinline__ void shifted16(const uint4 &v0, const uint4 &v1, int shift, uint32_t (&w)[4]) {
+    const uint32_t in[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+    const int words = shift >> 2, bits = (shift & 3) * 8;
+    uint32_t s[5];
+#pragma unroll
+    for (int i = 0; i < 5; i++) s[i] = words == 0 ? in[i] : words == 1 ? in[i + 1] : words == 2 ? in[i + 2] : (i + 3 < 8 ? in[i + 3] : 0u);
+#pragma unroll
+    for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(s[i], s[i + 1], bits);
+}
 // the 16 bytes at p, which need not be aligned; [lo, hi): the bytes that may be read in whole words around them
 template <typename T>
 __device__ __forceinline__ void load16(const uint8_t *p, const uint8_t *row_end, const uint8_t *lo, const uint8_t *hi, uint32_t (&w)[4]) {
@@ -89,13 +99,7 @@ __device__ __forceinline__ void load16(const uint8_t *p, const uint8_t *row_end,
     const uint8_t *const a = p - shift;
     if (p + 16 <= row_end && a >= lo && a + 32 <= hi) {
         const uint4 v0 = *(const uint4 *)a, v1 = *(const uint4 *)(a + 16);
-        const uint32_t in[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
-        const int words = shift >> 2, bits = (shift & 3) * 8;   // the same for a whole row
-        uint32_t s[5];
-#pragma unroll
-        for (int i = 0; i < 5; i++) s[i] = words == 0 ? in[i] : words == 1 ? in[i + 1] : words == 2 ? in[i + 2] : (i + 3 < 8 ? in[i + 3] : 0u);
-#pragma unroll
-        for (int i = 0; i < 4; i++) w[i] = __funnelshift_r(s[i], s[i + 1], bits);
+        shifted16(v0, v1, shift, w);
         return;
     }
     // value by value at the tensor's ends
@@ -132,10 +136,11 @@ struct Unpack {
 
 // EPT values a thread, a vector of 16 bytes at a time: value N j + i of vector v of thread t is element chunk * BS_NT * EPT + (v * BS_NT + t) * N + i
 template <typename T, int EPT>
-__global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
+__global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a) {
     constexpr int N = Unpack<T>::N, VECS = EPT / N;
     pdl_trigger();
     __shared__ __align__(16) float group_top[32];
+    __shared__ float bound_s;
     __shared__ double warp_sum[BS_NT / 32];
     __shared__ uint64_t list[BS_LIST];       // order of the value, then the complement of the token: larger is better
     __shared__ int n_list, part[BS_NT / 32];
@@ -147,16 +152,32 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
     const uint8_t *const base = a.logits + row * a.ld * (int64_t)sizeof(T), *const row_end = base + a.n_vocab * (int64_t)sizeof(T);
     const int first = chunk * BS_NT * EPT;   // the vocabulary is below 2^31
     float x[EPT];
-    if ((int64_t)first + BS_NT * EPT <= a.n_vocab && ((uintptr_t)base & 15) == 0) {
+    const bool whole = (int64_t)first + BS_NT * EPT <= a.n_vocab;
+    const int shift = (int)((uintptr_t)base & 15);
+    const uint8_t *const from = base - shift + (int64_t)first * (int)sizeof(T);   // whole vectors around the chunk
+    if (whole && shift == 0) {
         uint4 w[VECS];
 #pragma unroll
-        for (int v = 0; v < VECS; v++) w[v] = ld_stream16(base + (first + (v * BS_NT + tid) * N) * (int64_t)sizeof(T));
+        for (int v = 0; v < VECS; v++) w[v] = ld_stream16(from + (v * BS_NT + tid) * 16);
 #pragma unroll
         for (int v = 0; v < VECS; v++) {
             const uint32_t u[4] = {w[v].x, w[v].y, w[v].z, w[v].w};
             Unpack<T>::get(u, x + v * N);
         }
-    } else {   // the row's end, and rows that begin anywhere
+    } else if (whole && from >= a.logits && from + (BS_NT * VECS + 1) * 16 <= a.logits_end) {   // a row that begins anywhere: the vector behind is a neighbour's, from L1
+        uint4 w[VECS], next[VECS];
+#pragma unroll
+        for (int v = 0; v < VECS; v++) {
+            w[v] = __ldg((const uint4 *)(from + (v * BS_NT + tid) * 16));
+            next[v] = __ldg((const uint4 *)(from + (v * BS_NT + tid + 1) * 16));
+        }
+#pragma unroll
+        for (int v = 0; v < VECS; v++) {
+            uint32_t u[4];
+            shifted16(w[v], next[v], shift, u);
+            Unpack<T>::get(u, x + v * N);
+        }
+    } else {   // the row's end, and the tensor's
 #pragma unroll
         for (int v = 0; v < VECS; v++) {
             const int64_t e = (int64_t)first + (int64_t)(v * BS_NT + tid) * N;
@@ -170,18 +191,19 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
             }
         }
     }
-    float mine = -INFINITY;
+    float mine = -INFINITY, four[EPT / 4];   // maxima of all its values, of each four
 #pragma unroll
-    for (int i = 0; i < EPT; i += 2) {
-        x[i] = fmaxf(x[i], -INFINITY);   // a NaN counts as -inf
-        x[i + 1] = fmaxf(x[i + 1], -INFINITY);
-        mine = max3(mine, x[i], x[i + 1]);
+    for (int i = 0; i < EPT; i += 4) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[i + e] = fmaxf(x[i + e], -INFINITY);   // a NaN counts as -inf
+        four[i / 4] = fmaxf(max3(x[i], x[i + 1], x[i + 2]), x[i + 3]);
+        mine = fmaxf(mine, four[i / 4]);
     }
-    // maxima of groups of 8 threads, then of the chunk
+    // maxima of 32 groups of 16 threads, then of the chunk
     float g = mine;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if ((tid & 7) == 0) group_top[tid >> 3] = g;
+    for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if ((tid & 15) == 0) group_top[tid >> 4] = g;
     if (tid == 0) n_list = 0;
     __syncthreads();
     const int lane = tid & 31;
@@ -205,19 +227,20 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
     if (lane == 0) warp_sum[tid >> 5] = ds;
-    // A bound that k values of the chunk reach and few more do.  Up to 32 candidates: the k-th largest of the 32 groups' maxima, which every warp ranks for
-    // itself (independent values: 22 above it with k = 16, 130 with 32).  More: bisected over the threads' maxima until few more than k of the 256 have one
-    // (at 192 about 355 values).  It lets every finite value pass where fewer than k maxima are finite
+    // A bound that k values of the chunk reach and few more do.  Up to 32 candidates: the k-th largest of the 32 groups' maxima
+    // (of independent values 22 lie above it with k = 16, 130 with 32).  More: bisected over the threads' maxima until few more than k of the 512 have one
+    // (at 192 about 240 values).  It lets every finite value pass where fewer than k maxima are finite
     float bound;
     if (a.k <= 32) {
-        int better = 0;
+        // sixteen threads a group, two comparisons each
+        const int j = 2 * (lane & 15), me = tid >> 4;
+        const float2 o = *(const float2 *)(group_top + j);
+        int better = (o.x > g || (o.x == g && j < me)) + (o.y > g || (o.y == g && j + 1 < me));
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-            const float4 o = *(const float4 *)(group_top + j);
-            better += (o.x > mine_g || (o.x == mine_g && j < lane)) + (o.y > mine_g || (o.y == mine_g && j + 1 < lane)) + (o.z > mine_g || (o.z == mine_g && j + 2 < lane)) +
-                      (o.w > mine_g || (o.w == mine_g && j + 3 < lane));
-        }
-        bound = __shfl_sync(0xffffffffu, mine_g, __ffs(__ballot_sync(0xffffffffu, better == a.k - 1)) - 1);
+        for (int s16 = 8; s16 > 0; s16 >>= 1) better += __shfl_xor_sync(0xffffffffu, better, s16);
+        if (better == a.k - 1) bound_s = g;   // sixteen threads, one value
+        __syncthreads();
+        bound = bound_s;
     } else {
         uint32_t lo = ORDER32_NONE + 1, top = order32(m);
         const uint32_t best = order32(mine);
@@ -236,14 +259,17 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
         bound = value32(lo);
     }
     bound = fmaxf(bound, LOWEST);
-    if (mine >= bound) {
+    // (hits counted by warp and stored without the additions' answers: more instructions, slower)
 #pragma unroll
-        for (int i = 0; i < EPT; i++)
-            if (x[i] >= bound) {
-                const int at = atomicAdd(&n_list, 1);
-                if (at < BS_LIST) list[at] = (uint64_t)order32(x[i]) << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
-            }
-    }
+    for (int f = 0; f < EPT / 4; f++)
+        if (four[f] >= bound) {
+#pragma unroll
+            for (int i = 4 * f; i < 4 * f + 4; i++)
+                if (x[i] >= bound) {
+                    const int at = atomicAdd(&n_list, 1);
+                    if (at < BS_LIST) list[at] = (uint64_t)order32(x[i]) << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
+                }
+        }
     __syncthreads();
     int n = n_list;
     if (n > BS_LIST) {           // too many reach it: the k-th largest value itself, and of its equals the first
@@ -280,12 +306,15 @@ __global__ void __launch_bounds__(BS_NT) beam_rows_kernel(const SelectArgs a) {
         n = n_list;
     }
     Cand *const out = a.cand + slot * a.k;
-    for (int i = tid; i < n; i += BS_NT) {
-        const uint64_t me = list[i];
+    for (int base_i = 0; base_i < n; base_i += BS_NT / 4) {   // four threads a value
+        const int i = base_i + (tid >> 2);
+        const uint64_t me = i < n ? list[i] : 0;
         int better = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; j++) better += list[j] > me;
-        if (better < a.k) out[better] = {value32((uint32_t)(me >> 32)), (int)~(uint32_t)me};
+#pragma unroll 4
+        for (int j = tid & 3; j < n; j += 4) better += list[j] > me;
+        better += __shfl_xor_sync(0xffffffffu, better, 1);
+        better += __shfl_xor_sync(0xffffffffu, better, 2);
+        if (i < n && (tid & 3) == 0 && better < a.k) out[better] = {value32((uint32_t)(me >> 32)), (int)~(uint32_t)me};
     }
     for (int i = n + tid; i < a.k; i += BS_NT) out[i] = {-INFINITY, 0};
     if (tid == BS_NT - 1) {
@@ -332,13 +361,13 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
     for (int u = 0; u < BS_HELD; u++) mine[u] = tid + u * BS_MERGE_NT < total ? cand[tid + u * BS_MERGE_NT] : Cand{-INFINITY, 0};
     for (int b = warp; b < a.n_beam; b += BS_MERGE_NT / 32) {
         const int64_t row = row0 + b;
+        float t = lane < a.chunks ? a.top[row * a.chunks + lane] : -INFINITY;   // of an ended beam whatever stands there: not used
+        double part_sum = lane < a.chunks ? a.sum[row * a.chunks + lane] : 0.0;
         const float score = a.scores[row];
         const bool off = !(score > -INFINITY), ended = a.done && a.done[row];   // off: -inf or NaN
         float m = -INFINITY;
         double s = 0.0;
         if (!ended) {
-            float t = lane < a.chunks ? a.top[row * a.chunks + lane] : -INFINITY;
-            double part_sum = lane < a.chunks ? a.sum[row * a.chunks + lane] : 0.0;
             m = t;
             for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, a.top[row * a.chunks + c]);
 #pragma unroll
@@ -397,16 +426,16 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
     }
     if (tid % width == 0) key[tid / width] = most;
     __syncthreads();
-    if (tid < groups) {
-        const uint64_t me = key[tid];
-        int better = 0;
-#pragma unroll 8
-        for (int j = 0; j < groups; j++) {
+    {
+        int better = 0;   // the threads of a group share the comparisons
+#pragma unroll 2
+        for (int j = tid % width; j < groups; j += width) {
             const uint64_t other = key[j];
-            better += other > me || (other == me && j < tid);
+            better += other > most || (other == most && j < tid / width);
         }
-        if (better == a.k - 1) bound_s = me;
-        if (better == 0) best_s = me;
+        for (int o = width / 2; o > 0; o >>= 1) better += __shfl_xor_sync(0xffffffffu, better, o);
+        if (better == a.k - 1) bound_s = most;
+        if (better == 0) best_s = most;
     }
     __syncthreads();
     uint64_t lo = bound_s > ORDER64_NONE ? bound_s : ORDER64_NONE + 1;
@@ -441,13 +470,16 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
         __syncthreads();
         n = n_list;
     }
-    for (int i = tid; i < n; i += BS_MERGE_NT) {
-        const uint64_t me = key[i];
-        const int64_t at = where[i];
+    for (int base_i = 0; base_i < n; base_i += BS_MERGE_NT / 8) {   // eight threads a candidate
+        const int i = base_i + (tid >> 3);
+        const uint64_t me = i < n ? key[i] : 0;
+        const int64_t at = i < n ? where[i] : 0;
         int better = 0;
-#pragma unroll 8
-        for (int j = 0; j < n; j++) better += key[j] > me || (key[j] == me && where[j] < at);
-        if (better < a.k) {
+#pragma unroll 2
+        for (int j = tid & 7; j < n; j += 8) better += key[j] > me || (key[j] == me && where[j] < at);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) better += __shfl_xor_sync(0xffffffffu, better, o);
+        if (i < n && (tid & 7) == 0 && better < a.k) {
             const int64_t e = r * a.k + better;
             const uint64_t bits = me >> 63 ? me & ~(1ull << 63) : ~me;
             const int b = (int)(at / a.n_vocab);
@@ -463,12 +495,13 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
     }
 }
 
-// values a thread: 32, or fewer where that would leave SMs without a chunk
-int select_ept(int64_t rows, int64_t n_vocab) {
-    const int sms = sm_count();
-    for (int ept = 32; ept > 8; ept /= 2)
+// values a thread: 16, or 8 where that would leave SMs without a chunk (and 4 of F32).  (256 threads with 32 values each were 24 warps an SM and waited more:
+// 64 rows of 128256 17.2 us)
+int select_ept(int64_t rows, int64_t n_vocab, int type) {
+    const int sms = sm_count(), least = type == B200_TYPE_F32 ? 4 : 8;
+    for (int ept = 16; ept > least; ept /= 2)
         if (rows * ((n_vocab + BS_NT * ept - 1) / (BS_NT * ept)) >= 2 * sms) return ept;
-    return 8;
+    return least;
 }
 
 struct SelectPlan {
@@ -484,7 +517,7 @@ int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
     B200_REQUIRE(g.k >= 1 && g.k <= BS_MAX_K, "beam_select: %d candidates (1 to %d)", g.k, BS_MAX_K);
     B200_REQUIRE(g.n_vocab >= 1 && g.n_vocab <= (1 << 24) && g.logits_ld >= g.n_vocab, "beam_select: a vocabulary of %lld in rows %lld apart (up to 2^24)", (long long)g.n_vocab, (long long)g.logits_ld);
     p->rows = (int64_t)g.n_request * g.n_beam;
-    p->ept = select_ept(p->rows, g.n_vocab);
+    p->ept = select_ept(p->rows, g.n_vocab, g.logits_type);
     p->chunks = (g.n_vocab + BS_NT * p->ept - 1) / (BS_NT * p->ept);
     B200_REQUIRE(p->rows <= 65535, "beam_select: %lld rows are too many for one launch", (long long)p->rows);
     B200_REQUIRE(p->chunks * g.k * g.n_beam < 0x7fffffffLL, "beam_select: too many candidates of a request");
@@ -499,11 +532,10 @@ int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
 template <typename T>
 int launch_rows(const SelectArgs &a, const SelectPlan &p, cudaStream_t s) {
     const dim3 grid((unsigned)p.chunks, (unsigned)p.rows);
-    switch (p.ept) {
-        case 32: return launch_pdl(beam_rows_kernel<T, 32>, grid, dim3(BS_NT), 0, s, a);
-        case 16: return launch_pdl(beam_rows_kernel<T, 16>, grid, dim3(BS_NT), 0, s, a);
-        default: return launch_pdl(beam_rows_kernel<T, 8>, grid, dim3(BS_NT), 0, s, a);
-    }
+    if (p.ept == 16) return launch_pdl(beam_rows_kernel<T, 16>, grid, dim3(BS_NT), 0, s, a);
+    if constexpr (sizeof(T) == 4)
+        if (p.ept == 4) return launch_pdl(beam_rows_kernel<T, 4>, grid, dim3(BS_NT), 0, s, a);
+    return launch_pdl(beam_rows_kernel<T, 8>, grid, dim3(BS_NT), 0, s, a);
 }
 
 }  // namespace
@@ -537,6 +569,7 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
     uint8_t *const ws = (uint8_t *)g.workspace;
     SelectArgs a;
     a.logits = (const uint8_t *)g.logits;
+    a.logits_end = a.logits + ((p.rows - 1) * g.logits_ld + g.n_vocab) * size;
     a.scores = g.scores;
     a.done = g.done;
     a.ld = g.logits_ld;
