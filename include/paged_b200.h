@@ -36,7 +36,7 @@ struct b200_paged_cache {
 
 /* Keys and values of n_tok tokens into the cache, keys (and queries) turned to their positions on the way: what ROPE of q and k and two SET_ROWS do
  * in four nodes (crates/llama/src/graph_arch.rs:171-190, 1173-1240).  Token t belongs at position pos[t] of sequence seq[t] (seq null: sequence t);
- * a negative position is a padding token: nothing of it is read or written.  Every value is computed in F32 and rounded once.  n_dims
+ * a negative position is a padding token: nothing of it is written.  Every value is computed in F32 and rounded once.  n_dims
  * channels of a head rotate, in pairs (2 i, 2 i + 1) (mode 0, NORMAL) or (i, i + n_dims / 2) (mode 2, NEOX); the others are copied.  rope: (cos, sin)
  * rows by position as b200_rope_table makes them (pair i of a row at 2 i and 2 i + 1), rope_ld floats apart.  Strides are bytes per
  * token and per head.  Queries (n_head 0: none) go to q_out in the cache's type; q_out may be q where types and strides are the same.  Two tokens

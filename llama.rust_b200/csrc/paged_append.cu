@@ -60,9 +60,10 @@ struct AppendArgs {
     int64_t rope_rows, rope_ld;
     int n_head, n_dims, neox;
     unsigned per_tok, units;         // threads of a token, of a head
-    int64_t total;
+    int64_t n_tok;
     int *err;
 };
+constexpr int AP_NT = 128;
 
 template <typename XT>
 __device__ __forceinline__ void load8(const XT *p, float (&v)[8]) {
@@ -77,6 +78,10 @@ __device__ __forceinline__ void load8(const XT *p, float (&v)[8]) {
 }
 template <>
 __device__ __forceinline__ void load8<float>(const float *p, float (&v)[8]) {
+    if (((uintptr_t)p & 31) == 0) {   // a sector at once
+        asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]) : "l"(p) : "memory");
+        return;
+    }
     const float4 a = *(const float4 *)p, b = *(const float4 *)(p + 4);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
@@ -91,71 +96,75 @@ __device__ __forceinline__ void turn(float &a, float &b, float c, float s) {
     b = __fmaf_rn(x0, s, __fmul_rn(x1, c));
 }
 
-// VEC: 16 channels a thread, else one pair
+// A thread has one unit of one head of one token (a CTA a token, or 128 units of it; two or four tokens a thread, their rows on the way together, took longer:
+// 58 and 68 us for 55).  VEC: a unit is 16 channels, else one pair
 template <typename XT, typename CT, bool VEC>
-__global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs a) {
+__global__ void __launch_bounds__(AP_NT) paged_append_kernel(const AppendArgs a) {
+    constexpr int W = VEC ? 8 : 1;
     pdl_trigger();
-    pdl_wait();
-    const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (id >= a.total) return;
-    const int64_t t = id / a.per_tok;
-    const unsigned in_tok = (unsigned)(id - t * a.per_tok), slot = in_tok / a.units, u = in_tok - slot * a.units;
-    const int32_t p = a.pos[t];
-    if (p < 0) return;
+    const unsigned in_tok = blockIdx.y * AP_NT + threadIdx.x, slot = in_tok / a.units, u = in_tok - slot * a.units;
+    if (in_tok >= a.per_tok) return;
+    const int64_t t = blockIdx.x;
     const int what = (int)slot < a.n_head ? 0 : (int)slot < a.n_head + a.cache.n_head_kv ? 1 : 2;
     const int h = what == 0 ? (int)slot : what == 1 ? (int)slot - a.n_head : (int)slot - a.n_head - a.cache.n_head_kv;
-    const XT *src = (const XT *)(a.x[what] + t * a.x_nb1[what] + h * a.x_nb2[what]);
+    const bool turns = what < 2 && 2 * W * (int)u < a.n_dims;
+    const int e0 = turns && a.neox ? W * u : 2 * W * u, e1 = turns && a.neox ? e0 + a.n_dims / 2 : e0 + W;
+    const XT *const src = (const XT *)(a.x[what] + t * a.x_nb1[what] + h * a.x_nb2[what]);
+    pdl_wait();
+    const int32_t p = a.pos[t], s = a.seq ? a.seq[t] : (int32_t)t;
+    float x0[W], x1[W];
+    if constexpr (VEC) {   // on the way before the position is known
+        load8<XT>(src + e0, x0);
+        load8<XT>(src + e1, x1);
+    } else {
+        x0[0] = paged_f32(src[e0]);
+        x1[0] = paged_f32(src[e1]);
+    }
+    if (p < 0) return;
     // where it goes; what has no place is left out, of a token as a whole
-    const int32_t s = a.seq ? a.seq[t] : (int32_t)t;
     const int64_t row = s >= 0 && s < a.cache.n_seq ? paged_row(a.cache, s, p) : -1;
     if (row < 0 || (a.n_dims > 0 && p >= a.rope_rows)) {
         if (in_tok == 0) atomicExch(a.err, ERR_PAGED);
         return;
     }
-    CT *dst = what == 0 ? (CT *)(a.q_out + t * a.q_out_nb1 + h * a.q_out_nb2) : (CT *)((what == 1 ? a.cache.k : a.cache.v) + row) + (int64_t)h * a.cache.d;
-    const float *table = a.rope + p * a.rope_ld;
+    CT *const dst = what == 0 ? (CT *)(a.q_out + t * a.q_out_nb1 + h * a.q_out_nb2) : (CT *)((what == 1 ? a.cache.k : a.cache.v) + row) + (int64_t)h * a.cache.d;
+    const float *const table = a.rope + p * a.rope_ld + 2 * W * u;
     if constexpr (VEC) {
-        const bool turns = what < 2 && 16 * (int)u < a.n_dims;
-        const int e0 = turns && a.neox ? 8 * u : 16 * u, e1 = turns && a.neox ? e0 + a.n_dims / 2 : e0 + 8;
-        float x0[8], x1[8];
-        load8<XT>(src + e0, x0);
-        load8<XT>(src + e1, x1);
         if (turns) {
-            float cs[16];
-            load8<float>(table + 16 * u, *(float(*)[8])cs);
-            load8<float>(table + 16 * u + 8, *(float(*)[8])(cs + 8));
+            float c0[8], c1[8];
+            load8<float>(table, c0);
+            load8<float>(table + 8, c1);
             if (a.neox) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) turn(x0[i], x1[i], cs[2 * i], cs[2 * i + 1]);
+                for (int e = 0; e < 4; e++) {
+                    turn(x0[e], x1[e], c0[2 * e], c0[2 * e + 1]);
+                    turn(x0[4 + e], x1[4 + e], c1[2 * e], c1[2 * e + 1]);
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    turn(x0[i], x0[i + 1], cs[i], cs[i + 1]);
-                    turn(x1[i], x1[i + 1], cs[8 + i], cs[8 + i + 1]);
+                for (int e = 0; e < 8; e += 2) {
+                    turn(x0[e], x0[e + 1], c0[e], c0[e + 1]);
+                    turn(x1[e], x1[e + 1], c1[e], c1[e + 1]);
                 }
             }
         }
         store8<CT>(dst + e0, x0);
         store8<CT>(dst + e1, x1);
     } else {
-        const bool turns = what < 2 && 2 * (int)u < a.n_dims;
-        const int e0 = turns && a.neox ? u : 2 * u, e1 = turns && a.neox ? e0 + a.n_dims / 2 : e0 + 1;
-        float x0 = paged_f32(src[e0]), x1 = paged_f32(src[e1]);
-        if (turns) turn(x0, x1, table[2 * u], table[2 * u + 1]);
-        dst[e0] = paged_from<CT>(x0);
-        dst[e1] = paged_from<CT>(x1);
+        if (turns) turn(x0[0], x1[0], table[0], table[1]);
+        dst[e0] = paged_from<CT>(x0[0]);
+        dst[e1] = paged_from<CT>(x1[0]);
     }
 }
 
 template <typename XT, typename CT>
-int launch_append(AppendArgs a, bool vec, int64_t n_tok, cudaStream_t s) {
+int launch_append(AppendArgs a, bool vec, cudaStream_t s) {
     a.units = (unsigned)(a.cache.d / (vec ? 16 : 2));
     a.per_tok = a.units * (unsigned)(a.n_head + 2 * a.cache.n_head_kv);
-    a.total = n_tok * a.per_tok;
-    const int64_t blocks = (a.total + 255) / 256;
-    B200_REQUIRE(blocks < 0x7fffffffLL, "paged_append: too many tokens for one launch");
-    if (vec) return launch_pdl(paged_append_kernel<XT, CT, true>, dim3((unsigned)blocks), dim3(256), 0, s, a);
-    return launch_pdl(paged_append_kernel<XT, CT, false>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+    const unsigned y = (a.per_tok + AP_NT - 1) / AP_NT;
+    B200_REQUIRE(y <= 65535, "paged_append: too many heads for one launch");
+    if (vec) return launch_pdl(paged_append_kernel<XT, CT, true>, dim3((unsigned)a.n_tok, y), dim3(AP_NT), 0, s, a);
+    return launch_pdl(paged_append_kernel<XT, CT, false>, dim3((unsigned)a.n_tok, y), dim3(AP_NT), 0, s, a);
 }
 
 }  // namespace
@@ -188,6 +197,7 @@ extern "C" int b200_paged_append(const struct b200_paged_append_args *args, void
     const char *names[3] = {"the cache", "k", "q_out"};
     for (int i = 0; i < 3; i++)
         if ((rc = paged_check_device(mem[i], "paged_append", names[i])) != B200_STATUS_SUCCESS) return rc;
+    a.n_tok = g.n_tok;
     a.pos = g.pos;
     a.seq = g.seq;
     a.x[0] = (const uint8_t *)g.q; a.x[1] = (const uint8_t *)g.k; a.x[2] = (const uint8_t *)g.v;
@@ -206,7 +216,7 @@ extern "C" int b200_paged_append(const struct b200_paged_append_args *args, void
     const bool vec = all % 16 == 0 && out % 16 == 0 && g.n_dims % 16 == 0 && (g.n_dims == 0 || (((uintptr_t)g.rope | (uint64_t)(g.rope_ld * 4)) & 15) == 0);
     const cudaStream_t s = (cudaStream_t)stream;
     const bool bf = g.cache.type == B200_TYPE_BF16;
-    if (g.x_type == B200_TYPE_F32) return bf ? launch_append<float, __nv_bfloat16>(a, vec, g.n_tok, s) : launch_append<float, __half>(a, vec, g.n_tok, s);
-    if (g.x_type == B200_TYPE_F16) return bf ? launch_append<__half, __nv_bfloat16>(a, vec, g.n_tok, s) : launch_append<__half, __half>(a, vec, g.n_tok, s);
-    return bf ? launch_append<__nv_bfloat16, __nv_bfloat16>(a, vec, g.n_tok, s) : launch_append<__nv_bfloat16, __half>(a, vec, g.n_tok, s);
+    if (g.x_type == B200_TYPE_F32) return bf ? launch_append<float, __nv_bfloat16>(a, vec, s) : launch_append<float, __half>(a, vec, s);
+    if (g.x_type == B200_TYPE_F16) return bf ? launch_append<__half, __nv_bfloat16>(a, vec, s) : launch_append<__half, __half>(a, vec, s);
+    return bf ? launch_append<__nv_bfloat16, __nv_bfloat16>(a, vec, s) : launch_append<__nv_bfloat16, __half>(a, vec, s);
 }
