@@ -3,6 +3,8 @@
 //   acc = sum_p w_p v_p,  sum = sum_p w_p,  w_p = exp2(scale log2(e) q k_p - m)       over the whole tiles of 128 positions that a row shares, per part
 //
 //   * A CTA takes up to 128 rows (sequence of the group, query head of the key head), or 256 as two blocks, and a part of the tiles.  Row r of a block is lane r of tensor memory.
+//     Up to 64 (32) rows stand there twice (four times): products of 128 rows cost the same whatever they hold, and each copy takes the exponentials of half (a quarter) of a
+//     tile's positions, its weights of the others zero, so that all four warps of a softmax group have work; the copies' outputs are added at the end.
 //   * K and V come in tiles of 128 positions by TMA, a box a page (or as much of a page as a tile holds), the pages' ids read a tile ahead; K is a K-major
 //     and V an MN-major B operand, so neither is transposed.  A page id out of range is loaded from behind the last page (zeros), and the part's rows are marked to be
 //     computed again without it.
@@ -25,8 +27,10 @@ constexpr int TC_ERR_WAIT = 4;
 constexpr float TC_MOST = 4096.0f;   // sum of a tile's weights up to which the maximum in use is kept
 static_assert(TC_FEW_REGS * TC_SM_WARP0 * 32 + TC_MANY_REGS * (TC_THREADS - TC_SM_WARP0 * 32) <= TC_REGS * TC_THREADS, "register shares");
 
-template <typename T, int D, bool TWO>
+template <typename T, int D, int ROWS>
 struct TcCfg {
+    static constexpr bool TWO = ROWS == 256;
+    static constexpr int BLOCK = TWO ? 128 : ROWS, COPIES = TC_M / BLOCK, COLS = TC_N / COPIES;   // rows of a block; its copies in the lanes of tensor memory; positions that each copy answers for
     static constexpr int CHUNKS = D / 64;               // 64 elements = one 128-byte swizzled box
     static constexpr int TILE = TC_N * D * 2, Q = TC_M * D * 2 * (TWO ? 2 : 1);
     static constexpr int SLOTS = D == 128 ? (TWO ? 4 : 5) : TC_SLOTS_MAX;
@@ -77,11 +81,18 @@ __device__ __forceinline__ float2 tc_ex2_pair(uint64_t y) {
     return make_float2(__uint_as_float(__float_as_uint(f.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(f.y) + (__float_as_uint(n.y) << 23)));
 }
 
-template <typename T, int D, bool TWO>
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                 "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
+}
+
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(TC_THREADS, 1)
 prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap, const PrefixArgs a, const TcArgs ta) {
-    using C = TcCfg<T, D, TWO>;
-    constexpr int ROWS = TWO ? 2 * TC_M : TC_M;
+    using C = TcCfg<T, D, ROWS>;
+    constexpr bool TWO = C::TWO;
+    constexpr int COPIES = C::COPIES, COLS = C::COLS;
     extern __shared__ __align__(1024) uint8_t tc_raw[];
     const int64_t shared_ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts;
     if (blockIdx.x >= shared_ctas) {
@@ -95,7 +106,6 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     static_assert(sizeof(TcShared) <= 256, "barriers");
     TcShared &sh = *(TcShared *)(tc_raw + C::Q + C::SLOTS * C::TILE);
     const uint32_t q_s = pa_smem(tc_raw), kv_s = q_s + C::Q;
-    uint8_t *const q_g = tc_raw;
     if (q_s & 1023u) {   // the swizzle counts in 1024 bytes
         pdl_wait();
         if (threadIdx.x == 0) atomicExch(a.err, TC_ERR_WAIT);
@@ -244,22 +254,22 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         const int g = (warp - TC_SM_WARP0) >> 2, r = (warp & 3) * 32 + lane;   // softmax group, row of its block: a warp reaches the tensor-memory lanes of its number modulo 4
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t t_s = tmem + lanes + (uint32_t)(g * TC_N), t_o = tmem + lanes + C::O_COL + (uint32_t)(g * D);
-        const int x = (TWO ? g * TC_M : 0) + r;
+        const int copy = r / C::BLOCK, x = TWO ? g * TC_M + r : r % C::BLOCK;
         const bool live = x < n_rows;
         const int seq = first + (live ? (x0 + x) / a.each : 0), head = hk * a.each + (live ? (x0 + x) % a.each : 0);
         const int64_t out = ((int64_t)seq * a.n_head + head) * (a.shared_parts + PX_WARPS * a.own_parts) + part;
         const int my_tiles = live ? min(prefix_cover(a, seq) / PX_TILE, n_all) - t0 : 0;   // tiles of this part that the row sees
         if (n_tiles > 0) {
-            // q into the swizzled K-major operand, zeros behind the last row: a warp takes ROWS / 8 rows, a lane 16 bytes at a time, all under way at once (row by row
+            // q into the swizzled K-major operand, zeros behind the last row: a warp takes an eighth of the rows, a lane 16 bytes at a time, all under way at once (row by row
             // through registers this took 14 us of a launch)
-            constexpr int LANES = D / 8, PER = 32 / LANES, RW = ROWS / 8;   // lanes of a row, rows at a time
+            constexpr int LANES = D / 8, PER = 32 / LANES, RW = (TWO ? 2 : 1) * TC_M / 8;   // lanes of a row, rows at a time
             const int e = lane % LANES, c = e >> 3, u = e & 7;
 #pragma unroll
             for (int h = 0; h < RW; h += PER) {
-                const int y = (warp - TC_SM_WARP0) * RW + h + lane / LANES, yb = y % TC_M, row = x0 + (y < n_rows ? y : 0), i = row / a.each;
+                const int y = (warp - TC_SM_WARP0) * RW + h + lane / LANES, yb = y % TC_M, yr = TWO ? y : y % C::BLOCK, row = x0 + (yr < n_rows ? yr : 0), i = row / a.each;
                 const uint8_t *const src = a.q + (int64_t)(first + i) * a.q_nb1 + (int64_t)(hk * a.each + row - i * a.each) * a.q_nb2 + 16 * e;
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(q_s + (uint32_t)((y / TC_M) * (TC_M * D * 2) + c * (TC_M * 128) + (yb >> 3) * 1024 + (yb & 7) * 128 + ((u ^ (yb & 7)) << 4))),
-                             "l"(src), "r"(y < n_rows ? 16 : 0)
+                             "l"(src), "r"(yr < n_rows ? 16 : 0)
                              : "memory");
             }
             asm volatile("cp.async.wait_all;" ::: "memory");
@@ -276,19 +286,20 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 pa_fence_after();
                 const bool sees = (TWO ? j : 2 * j + g) < my_tiles;
                 const float sc = a.scale_log2;
-                uint32_t p[TC_N / 2];
+                uint32_t p[COLS / 2];
+                const uint32_t t_mine = t_s + (uint32_t)(copy * COLS);   // the warp's: a copy's rows are whole warps
                 // the weights under the maximum in use; where their sum says that it has grown too much, and where there is none yet, once more under the tile's own
                 bool anew = __any_sync(0xffffffffu, sees && m == -INFINITY);
                 for (;;) {
-                    uint32_t s[TC_N];
+                    uint32_t s[COLS];
 #pragma unroll
-                    for (int c = 0; c < TC_N; c += 32) pa_ld32(s + c, t_s + (uint32_t)c);
+                    for (int c = 0; c < COLS; c += 32) pa_ld32(s + c, t_mine + (uint32_t)c);
                     pa_wait_ld();
                     if (anew) {
                         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         const float sign = sc < 0.0f ? -1.0f : 1.0f;   // under a negative scale the smallest score is the largest
 #pragma unroll
-                        for (int c = 0; c < TC_N; c += 4)
+                        for (int c = 0; c < COLS; c += 4)
 #pragma unroll
                             for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], sign * __uint_as_float(s[c + e]));
                         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
@@ -314,7 +325,7 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     const float sub = m == -INFINITY ? 0.0f : -m;
                     const uint64_t sc2 = pa_pair(sc, sc), sub2 = pa_pair(sub, sub);
 #pragma unroll
-                    for (int c = 0; c < TC_N / 2; c++) {
+                    for (int c = 0; c < COLS / 2; c++) {
                         const uint64_t y = pa_fma2(pa_pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, sub2);
                         const float2 e = (c * 3) % 8 < 3 ? tc_ex2_pair(y) : tc_ex2_units(y);
                         p[c] = paged_pack<T>(e.x, e.y);
@@ -331,10 +342,20 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 }
                 if (!sees || m == -INFINITY) {   // weights of zero, whatever the scores were
 #pragma unroll
-                    for (int c = 0; c < TC_N / 2; c++) p[c] = 0u;
+                    for (int c = 0; c < COLS / 2; c++) p[c] = 0u;
                 }
-                pa_st32(t_s, p);
-                pa_st32(t_s + 32u, p + 32);
+                if constexpr (COPIES == 4) {
+                    const uint32_t none[16] = {};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) tc_st16(t_s + (uint32_t)(16 * c), c == copy ? p : none);
+                } else if constexpr (COPIES == 2) {
+                    const uint32_t none[32] = {};
+#pragma unroll
+                    for (int c = 0; c < 2; c++) pa_st32(t_s + (uint32_t)(32 * c), c == copy ? p : none);
+                } else {
+                    pa_st32(t_s, p);
+                    pa_st32(t_s + 32u, p + 32);
+                }
                 pa_wait_st();
                 pa_fence_before();
             }
@@ -343,15 +364,19 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
         }
         if (l != l) m = fmaxf(m, 0.0f);   // a NaN score is no maximum, but the row has seen it
         if (n_tiles == 0) {
-            if (live && (TWO || g == 0)) a.ml[out] = make_float2(-INFINITY, 0.0f);
+            if (live && copy == 0 && (TWO || g == 0)) a.ml[out] = make_float2(-INFINITY, 0.0f);
         } else {
             const bool finished = __all_sync(0xffffffffu, pa_wait(&sh.done, 0, abort_flag, ta.wait_limit) && !*abort_flag);
             pa_fence_after();
+            // All products are through, or nothing will be stored: the operands' memory takes maxima and sums (over the queries) and the outputs (over the slots, row
+            // after row, 16-byte piece u of row y at u ^ (y % 32)), so that rows go out whole
+            float2 *const ml = (float2 *)tc_raw, *const fin = ml + 2 * TC_M;   // of both softmax groups, of a lane
+            int64_t *const outs = (int64_t *)(fin + TC_M);
+            float4 *const rows = (float4 *)(tc_raw + C::Q);
             float wa = 1.0f, wb = 0.0f;
             bool ina = m != -INFINITY, inb = false;
             int c0 = 0, c1 = D;
             if (!TWO) {   // the two groups' outputs under their common maximum, half the channels each
-                float2 *const ml = (float2 *)(q_g + C::Q);   // [2][TC_M] in the first slot: its last product is through, or nothing of it will be stored
                 ml[g * TC_M + r] = make_float2(m, l);
                 asm volatile("bar.sync 1, 256;" ::: "memory");
                 const float2 la = ml[r], lb = ml[TC_M + r];
@@ -364,29 +389,60 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                 l = (ina ? wa * la.y : 0.0f) + (inb ? wb * lb.y : 0.0f);
                 c0 = g * (D / 2);
                 c1 = c0 + D / 2;
+                if (COPIES > 1) {   // the copies' too
+                    if (g == 0) fin[r] = make_float2(m, l);
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+                    for (int q = 0; q < COPIES; q++) top = fmaxf(top, fin[q * C::BLOCK + x].x);
+#pragma unroll
+                    for (int q = 0; q < COPIES; q++) {
+                        const float2 f = fin[q * C::BLOCK + x];
+                        if (f.x != -INFINITY) sum += pa_ex2(f.x - top) * f.y;
+                    }
+                    const float f = m == -INFINITY ? 0.0f : pa_ex2(m - top);
+                    wa *= f;
+                    wb *= f;
+                    m = top;
+                    l = sum;
+                }
             }
-            if (live && c0 == 0) a.ml[out] = !finished ? make_float2(NAN, NAN) : *(volatile int *)&sh.bad ? make_float2(NAN, 0.0f) : make_float2(m, l);
-            if (finished && warp_live) {
-                float *const dst = a.acc + out * D;
+            if (copy == 0 && c0 == 0) {
+                outs[x] = live ? out : -1;
+                if (live) a.ml[out] = !finished ? make_float2(NAN, NAN) : *(volatile int *)&sh.bad ? make_float2(NAN, 0.0f) : make_float2(m, l);
+            }
+            const int y = TWO ? g * TC_M + r : r;
+            if (warp_live) {
 #pragma unroll 1
                 for (int c = c0; c < c1; c += 32) {
                     uint32_t u[32], v[TWO ? 1 : 32];
                     pa_ld32(u, tmem + lanes + C::O_COL + (uint32_t)((TWO ? g * D : 0) + c));
                     if constexpr (!TWO) pa_ld32(v, tmem + lanes + C::O_COL + (uint32_t)(D + c));
                     pa_wait_ld();
-                    if (live && m != -INFINITY) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            float z = __uint_as_float(u[e]);
-                            if constexpr (!TWO) z = (ina ? wa * z : 0.0f) + (inb ? wb * __uint_as_float(v[e]) : 0.0f);
-                            u[e] = __float_as_uint(z);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8)
-                            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(dst + c + e), "r"(u[e]), "r"(u[e + 1]), "r"(u[e + 2]), "r"(u[e + 3]), "r"(u[e + 4]), "r"(u[e + 5]), "r"(u[e + 6]),
-                                         "r"(u[e + 7])
-                                         : "memory");
+                    for (int e = 0; e < 32; e++) {
+                        float z = ina ? (TWO ? __uint_as_float(u[e]) : wa * __uint_as_float(u[e])) : 0.0f;
+                        if constexpr (!TWO) z += inb ? wb * __uint_as_float(v[e]) : 0.0f;
+                        u[e] = __float_as_uint(z);
                     }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        rows[y * (D / 4) + (((c + e) / 4) ^ (y & (D / 4 - 1)))] = make_float4(__uint_as_float(u[e]), __uint_as_float(u[e + 1]), __uint_as_float(u[e + 2]), __uint_as_float(u[e + 3]));
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (!*abort_flag) {
+                const int n = min(n_rows, TWO ? 2 * TC_M : C::BLOCK);
+                for (int i = tid - TC_SM_WARP0 * 32; i < n * (D / 4); i += 256) {
+                    const int z = i / (D / 4), u = i % (D / 4);
+                    float4 f = rows[z * (D / 4) + (u ^ (z & (D / 4 - 1)))];
+#pragma unroll
+                    for (int q = 1; q < COPIES; q++) {
+                        const int zq = q * C::BLOCK + z;
+                        const float4 h = rows[zq * (D / 4) + (u ^ (zq & (D / 4 - 1)))];
+                        f.x += h.x; f.y += h.y; f.z += h.z; f.w += h.w;
+                    }
+                    *(float4 *)(a.acc + outs[z] * D + 4 * u) = f;
                 }
             }
         }
@@ -398,9 +454,9 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     if (*abort_flag && tid == 0) atomicExch(a.err, TC_ERR_WAIT);
 }
 
-template <typename T, int D, bool TWO>
+template <typename T, int D, int ROWS>
 int launch(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
-    using C = TcCfg<T, D, TWO>;
+    using C = TcCfg<T, D, ROWS>;
     TcArgs ta;
     attn_wait_hook(&ta.wait_limit, &ta.mute);
     const int page = 1 << a.cache.page_log2;
@@ -409,29 +465,34 @@ int launch(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
     B200_REQUIRE(paged_tile_map(&km, type, a.cache.k, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box) &&
                      paged_tile_map(&vm, type, a.cache.v, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box),
                  "prefix_attn: tensor maps over %lld pages of %d positions refused", (long long)a.cache.n_pages, page);
-    B200_CUDA(cudaFuncSetAttribute(prefix_parts_kernel<T, D, TWO>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    B200_CUDA(cudaFuncSetAttribute(prefix_parts_kernel<T, D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     // the warps' register shares come out of what the block is launched with
     static const int regs = [] {
         cudaFuncAttributes fa;
-        return cudaFuncGetAttributes(&fa, prefix_parts_kernel<T, D, TWO>) == cudaSuccess ? fa.numRegs : 0;
+        return cudaFuncGetAttributes(&fa, prefix_parts_kernel<T, D, ROWS>) == cudaSuccess ? fa.numRegs : 0;
     }();
     B200_REQUIRE(regs >= TC_REGS, "prefix_attn: a build with %d registers a thread cannot share them out", regs);
     const int64_t ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts + a.own_ctas;
-    return launch_pdl(prefix_parts_kernel<T, D, TWO>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
+    return launch_pdl(prefix_parts_kernel<T, D, ROWS>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
 }
 
 }  // namespace
 
-int prefix_shared_rows(int64_t rows) { return rows > TC_M ? 2 * TC_M : TC_M; }
+int prefix_shared_rows(int64_t rows) { return rows > 128 ? 256 : rows > 64 ? 128 : rows > 32 ? 64 : 32; }
+
+template <typename T, int D>
+static int launch_rows(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
+    switch (prefix_shared_rows((int64_t)a.served * a.each)) {
+        case 32: return launch<T, D, 32>(a, type, s);
+        case 64: return launch<T, D, 64>(a, type, s);
+        case 128: return launch<T, D, 128>(a, type, s);
+        default: return launch<T, D, 256>(a, type, s);
+    }
+}
 
 int launch_prefix_parts(const PrefixArgs &a, int type, cudaStream_t s) {
-    const bool two = prefix_shared_rows((int64_t)a.served * a.each) == 2 * TC_M;
-    if (type == B200_TYPE_F16) {
-        if (a.cache.d == 128) return two ? launch<__half, 128, true>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s) : launch<__half, 128, false>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s);
-        return two ? launch<__half, 64, true>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s) : launch<__half, 64, false>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s);
-    }
-    if (a.cache.d == 128) return two ? launch<__nv_bfloat16, 128, true>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s) : launch<__nv_bfloat16, 128, false>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s);
-    return two ? launch<__nv_bfloat16, 64, true>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s) : launch<__nv_bfloat16, 64, false>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s);
+    if (type == B200_TYPE_F16) return a.cache.d == 128 ? launch_rows<__half, 128>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s) : launch_rows<__half, 64>(a, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, s);
+    return a.cache.d == 128 ? launch_rows<__nv_bfloat16, 128>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s) : launch_rows<__nv_bfloat16, 64>(a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, s);
 }
 
 }  // namespace b200
