@@ -373,8 +373,11 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             for (int c = lane;;) {
-                // exp(t - m), and 2^-(t log2(e) - its rounding) for the chunk's sum
-                if (t > -INFINITY) s += part_sum * (fabsf(t) < 1e30f ? (double)fast_exp2(t == m ? -fmaf(t, LOG2E, -(t * LOG2E)) : (t - m) * LOG2E - fmaf(t, LOG2E, -(t * LOG2E))) : t == m ? 1.0 : exp((double)t - (double)m));
+                // exp(t - m), and what c = t log2(e) was off by when the chunk's exponentials were taken
+                if (t > -INFINITY) {
+                    const double back = fabsf(t) < 1e30f ? 1.0 - 0.6931471805599453 * (double)fmaf(t, LOG2E, -(t * LOG2E)) : 1.0;
+                    s += part_sum * back * (t == m ? 1.0 : fabsf(m) < 1e30f ? (double)fast_exp2((t - m) * LOG2E) : exp((double)t - (double)m));
+                }
                 c += 32;
                 if (c >= a.chunks) break;
                 t = a.top[row * a.chunks + c];

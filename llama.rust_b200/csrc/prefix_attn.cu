@@ -139,8 +139,9 @@ struct PrefixPlan {
 
 // Into how many parts the positions are cut, and how the SMs are dealt out between the shared part (a CTA a part, one an SM, first) and the own part
 // (CTAs that walk the items, three at a time): what takes least by a model of the launch.  Times in ns, measured with 8 key heads of 128 and of 64
-// channels: a CTA of the shared part about 10000 and, a tile, 1850 with two blocks of rows, 5500 and 1300 (an SM takes in 50 GB/s) with one; a unit of the own part 4000, 700
-// an item and, a tile, 650 for each of the SM's units (the same 50 GB/s), at least 1000; a row's partial output crosses L2 twice at about 5 bytes a picosecond.
+// channels: a CTA of the shared part about 10000 and, a tile, 1850 with two blocks of rows, 6000 and 1250 with one (5000 and 850 with 64 channels); a unit of the own part
+// 4000, 1500 an item and, a tile, 580 for each of the SM's units (an SM takes in 50 GB/s), at least 900; a row's partial output crosses L2 twice at about 5 bytes a
+// picosecond.
 struct PartsPlan {
     int64_t d, rows, shared_items, shared_tiles, own_items, own_tiles;
     bool two_blocks;
@@ -149,7 +150,7 @@ struct PartsPlan {
 void plan_parts(PartsPlan *p, int64_t sms) {
     static const int counts[] = {1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 11, 12, 14, 16, 18, 24, 32, 48, 64};
     static_assert(PX_MAX_PARTS == 64, "the most parts there are");
-    const int64_t wide = p->d == 128, c_shared = p->two_blocks ? (wide ? 1850 : 1300) : (wide ? 1300 : 950), f_shared = p->two_blocks ? 10000 : 5500;
+    const int64_t wide = p->d == 128, c_shared = p->two_blocks ? (wide ? 1850 : 1300) : (wide ? 1250 : 850), f_shared = p->two_blocks ? 10000 : wide ? 6000 : 5000;
     int64_t best = INT64_MAX;
     p->shared_parts = p->own_parts = p->own_ctas = 1;
     if (p->own_items == 0) return;
@@ -161,8 +162,8 @@ void plan_parts(PartsPlan *p, int64_t sms) {
         for (int no : counts) {
             if (no > 1 && no > p->own_tiles) break;
             const int64_t items = p->own_items * no, ctas = items < left ? items : left, units = items < 3 * ctas ? (items + ctas - 1) / ctas : 3;
-            const int64_t each = (items + ctas * units - 1) / (ctas * units), tile = (wide ? 650 : 325) * units > 1000 ? (wide ? 650 : 325) * units : 1000;
-            const int64_t t2 = 4000 + each * (700 + tile * ((p->own_tiles + no - 1) / no));
+            const int64_t each = (items + ctas * units - 1) / (ctas * units), tile = (wide ? 580 : 290) * units > 900 ? (wide ? 580 : 290) * units : 900;
+            const int64_t t2 = 4000 + each * ((wide ? 1500 : 1000) + tile * ((p->own_tiles + no - 1) / no));
             const int64_t shared = (waves + (n1 > waves * sms)) * t1, own = waves * t1 + t2;
             const int64_t time = (shared > own ? shared : own) + p->rows * (PX_WARPS * no + (n1 ? ns : 0)) * p->d * 8 / 5000;
             if (time < best) {

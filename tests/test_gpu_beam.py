@@ -71,6 +71,27 @@ def test_many_rows_take_long_chunks(p):
     select(p, head(rng, 40, 4, 20011, "BF16"), -5 * rng.random((40, 4)), 8, "BF16")
 
 
+def test_a_large_vocabulary(p):
+    rng = np.random.default_rng(12)
+    select(p, head(rng, 1, 2, 1000003), -rng.random((1, 2)), 128)
+    select(p, head(rng, 1, 2, 1000003, "F16"), -rng.random((1, 2)), 4, "F16")
+
+
+@pytest.mark.parametrize("offset", [0.0, 30.0, -500.0, 2000.0])
+def test_logits_far_from_zero(p, offset):
+    # x log2(e) is rounded once for a chunk's maximum: what that is off by must not show
+    rng = np.random.default_rng(13)
+    x = P.rounded(head(rng, 2, 3, 20000) + offset, "F32")
+    select(p, x, -rng.random((2, 3)), 8)
+
+
+def test_one_word_has_nearly_all_the_probability(p):
+    rng = np.random.default_rng(14)
+    x = head(rng, 2, 3, 9000)
+    x[:, :, 4321] = 60.0
+    select(p, P.rounded(x, "F32"), -rng.random((2, 3)), 6)
+
+
 @pytest.mark.parametrize("ty,V,pad,off", [("F32", 999, 1, 0), ("F32", 999, 0, 1), ("F32", 1024, 2, 3), ("BF16", 999, 1, 1), ("BF16", 1003, 0, 7), ("F16", 4096, 5, 3), ("BF16", 4095, 0, 0)])
 def test_rows_at_any_address(p, ty, V, pad, off):
     rng = np.random.default_rng(V)

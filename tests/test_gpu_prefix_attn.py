@@ -135,6 +135,84 @@ def test_row_blocks_that_are_not_whole(p, each, n):
     Problem(p, [n, 2], [400 + i % 50 for i in range(n + 2)], [390] * (n + 2), "BF16", 128, 1, each, 64).run()
 
 
+@pytest.mark.parametrize("rows", [31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257])
+@pytest.mark.parametrize("ty,d", [("F16", 64), ("BF16", 128)])
+def test_blocks_of_every_kind_at_their_borders(p, rows, ty, d):
+    # every form of the shared part (32, 64, 128, 256 rows a block) full, one short and one over; several tiles, rows that see fewer
+    lens = [540 - (i % 5) * 128 for i in range(rows)]
+    Problem(p, [rows], lens, [520] * rows, ty, d, 1, 1, 32, seed=rows).run()
+
+
+@pytest.mark.parametrize("n,each", [(8, 4), (16, 4), (30, 4), (60, 4)])
+def test_scores_that_grow_along_the_positions(p, n, each):
+    # the maximum in use falls behind again and again: by little, by more than 2^12, and all at once
+    for dev in (0.02, 0.3, 4.0):
+        pr = Problem(p, [n], [900] * n, [896] * n, "BF16", 64, 1, each, 128)
+        page, place = np.array([P.cell(pr.tables.tolist(), 0, x, 128, pr.n_pages) for x in range(896)]).T
+        pr.q[:, :, 0] = 1.0
+        pr.k[page, place, 0, 0] = P.rounded(np.arange(896) * dev, "BF16")
+        pr.run()
+
+
+def test_a_few_positions_outweigh_all_others(p):
+    for at in (0, 127, 128, 500, 767):
+        pr = Problem(p, [9], [800] * 9, [768] * 9, "F16", 128, 2, 4, 64)
+        page, place = P.cell(pr.tables.tolist(), 0, at, 64, pr.n_pages)
+        pr.k[page, place] = P.rounded(pr.k[page, place] * 12, "F16")
+        pr.run()
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("n", [2, 14, 30, 70])
+def test_infinities_that_all_rows_see(p, value, n):
+    pr = Problem(p, [n], [300 + i for i in range(n)], [256] * n, "BF16", 64, 1, 4, 16)
+    page, place = P.cell(pr.tables.tolist(), 0, 77, 16, pr.n_pages)
+    pr.v[page, place, 0, 9] = value
+    pr.run()
+
+
+def test_more_groups_than_the_gpu_has_multiprocessors(p):
+    n = 340
+    Problem(p, [2] * 170, [150 + i % 40 for i in range(n)], [140] * n, "F16", 64, 1, 2, 16).run()
+
+
+def test_many_heads_a_key_head(p):
+    Problem(p, [3], [400, 390, 380], [384] * 3, "BF16", 64, 2, 100, 64, sinks=True).run()
+
+
+def test_bad_pages_of_the_shared_part_in_every_form(p):
+    for n in (4, 12, 28, 70):
+        pr = Problem(p, [n], [420 + i % 7 for i in range(n)], [400] * n, "BF16", 128, 1, 4, 32)
+        pr.tables[0, 5] = pr.n_pages
+        pr.run(error=7)
+
+
+@pytest.mark.parametrize("n", [5, 14, 30, 70])
+def test_a_wait_that_runs_out(p, n):
+    """the first CTA of the shared part never asks for its first values: its rows stay as they were, the others' results are those of an undisturbed call"""
+    m = b200.load()
+    pr = Problem(p, [n, 3], [700 + i for i in range(n + 3)], [640] * (n + 3), "BF16", 128, 2, 4, 64)
+    call = pr.call()
+    call(None)
+    good = pr.result()
+    assert m.kernel_error() == 0
+    pr.out.upload(P.bits(np.full(pr.q.size + GUARD, -7.0), "BF16"))
+    m.lib.b200_debug_attn_wait(20000, 0)
+    try:
+        call(None)
+        m.synchronize()
+    finally:
+        m.lib.b200_debug_attn_wait(0, -1)
+    assert m.kernel_error() == 4 and m.kernel_error() == 0
+    got = pr.result()
+    rows = min(n, 64)   # of the first block: at most 256 rows of 4 query heads
+    assert (got[:rows, :4] == -7.0).all()
+    got[:rows, :4] = good[:rows, :4]
+    assert np.array_equal(got, good)
+    call(None)
+    assert np.array_equal(pr.result(), good) and m.kernel_error() == 0
+
+
 def test_own_positions_are_long(p):
     Problem(p, [2, 2], [2000, 1500, 90, 2222], [40] * 4, "BF16", 128, 2, 4, 16).run()
 

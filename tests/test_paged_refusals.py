@@ -55,7 +55,7 @@ def refused(call, words):
 @pytest.mark.parametrize("kw,words", [
     (dict(ty=0), "neither F16 nor BF16"), (dict(page_size=8), "pages of 8"), (dict(page_size=48), "pages of 48"), (dict(page_size=512), "pages of 512"), (dict(n_head_kv=0), "key heads"), (dict(d=72), "72 channels"),
     (dict(d=2048), "2048 channels"), (dict(d=0), "0 channels"), (dict(k=None), "null cache"), (dict(v=A + 8), "16-byte aligned"), (dict(tables=None), "null cache"), (dict(n_pages=0), "empty"),
-    (dict(table_ld=0), "empty"), (dict(n_seq=0), "empty"), (dict(page_stride=2048), "page stride"), (dict(page_stride=16 * 256 + 8), "page stride")])
+    (dict(table_ld=0), "empty"), (dict(table_ld=1 << 31), "too large"), (dict(page_stride=1 << 40), "page stride"), (dict(n_seq=0), "empty"), (dict(page_stride=2048), "page stride"), (dict(page_stride=16 * 256 + 8), "page stride")])
 def test_cache_arguments(p, kw, words):
     refused(append_of(p, cache_of(p, **kw)), words)
     refused(attn_of(p, cache_of(p, **kw)), words)
