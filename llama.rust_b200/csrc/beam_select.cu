@@ -22,6 +22,7 @@ namespace {
 
 constexpr int BS_NT = 512, BS_MAX_K = 128, BS_MAX_BEAM = 64;
 constexpr int BS_LIST = 512;            // candidates that are ordered by counting
+constexpr int BS_CLUSTER = 16;          // chunks of a request that one launch takes
 constexpr int BS_MERGE_NT = 512, BS_HELD = 4;   // threads of the merge; candidates each keeps in registers
 
 struct Cand {                            // of a chunk, in descending order; behind its last one -inf
@@ -134,21 +135,20 @@ struct Unpack {
     }
 };
 
-// EPT values a thread, a vector of 16 bytes at a time: value N j + i of vector v of thread t is element chunk * BS_NT * EPT + (v * BS_NT + t) * N + i
+struct ChunkShared {
+    __align__(16) float group_top[32];
+    float bound;
+    double warp_sum[BS_NT / 32];
+    uint64_t list[BS_LIST];                  // order of the value, then the complement of the token: larger is better
+    int n_list, part[BS_NT / 32];
+};
+
+// A chunk of a row: its k best (behind the last one -inf), its maximum, its sum of exponentials.  EPT values a thread, a vector of 16 bytes at a time: value N j + i of
+// vector v of thread t is element chunk * BS_NT * EPT + (v * BS_NT + t) * N + i
 template <typename T, int EPT>
-__global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a) {
+__device__ __forceinline__ void beam_chunk(const SelectArgs &a, int64_t row, int chunk, Cand *out, float *out_top, double *out_sum, ChunkShared &sh) {
     constexpr int N = Unpack<T>::N, VECS = EPT / N;
-    pdl_trigger();
-    __shared__ __align__(16) float group_top[32];
-    __shared__ float bound_s;
-    __shared__ double warp_sum[BS_NT / 32];
-    __shared__ uint64_t list[BS_LIST];       // order of the value, then the complement of the token: larger is better
-    __shared__ int n_list, part[BS_NT / 32];
-    const int tid = threadIdx.x, chunk = blockIdx.x;
-    const int64_t row = blockIdx.y;
-    const int64_t slot = row * a.chunks + chunk;
-    pdl_wait();
-    if (a.done && a.done[row]) return;       // the merge does not ask for this beam
+    const int tid = threadIdx.x;
     const uint8_t *const base = a.logits + row * a.ld * (int64_t)sizeof(T), *const row_end = base + a.n_vocab * (int64_t)sizeof(T);
     const int first = chunk * BS_NT * EPT;   // the vocabulary is below 2^31
     float x[EPT];
@@ -203,11 +203,11 @@ __global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a)
     float g = mine;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
-    if ((tid & 15) == 0) group_top[tid >> 4] = g;
-    if (tid == 0) n_list = 0;
+    if ((tid & 15) == 0) sh.group_top[tid >> 4] = g;
+    if (tid == 0) sh.n_list = 0;
     __syncthreads();
     const int lane = tid & 31;
-    const float mine_g = group_top[lane];
+    const float mine_g = sh.group_top[lane];
     float m = mine_g;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a)
     double ds = (double)s;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
-    if (lane == 0) warp_sum[tid >> 5] = ds;
+    if (lane == 0) sh.warp_sum[tid >> 5] = ds;
     // A bound that k values of the chunk reach and few more do.  Up to 32 candidates: the k-th largest of the 32 groups' maxima
     // (of independent values 22 lie above it with k = 16, 130 with 32).  More: bisected over the threads' maxima until few more than k of the 512 have one
     // (at 192 about 240 values).  It lets every finite value pass where fewer than k maxima are finite
@@ -234,13 +234,13 @@ __global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a)
     if (a.k <= 32) {
         // sixteen threads a group, two comparisons each
         const int j = 2 * (lane & 15), me = tid >> 4;
-        const float2 o = *(const float2 *)(group_top + j);
+        const float2 o = *(const float2 *)(sh.group_top + j);
         int better = (o.x > g || (o.x == g && j < me)) + (o.y > g || (o.y == g && j + 1 < me));
 #pragma unroll
         for (int s16 = 8; s16 > 0; s16 >>= 1) better += __shfl_xor_sync(0xffffffffu, better, s16);
-        if (better == a.k - 1) bound_s = g;   // sixteen threads, one value
+        if (better == a.k - 1) sh.bound = g;   // sixteen threads, one value
         __syncthreads();
-        bound = bound_s;
+        bound = sh.bound;
     } else {
         uint32_t lo = ORDER32_NONE + 1, top = order32(m);
         const uint32_t best = order32(mine);
@@ -266,12 +266,12 @@ __global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a)
 #pragma unroll
             for (int i = 4 * f; i < 4 * f + 4; i++)
                 if (x[i] >= bound) {
-                    const int at = atomicAdd(&n_list, 1);
-                    if (at < BS_LIST) list[at] = (uint64_t)order32(x[i]) << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
+                    const int at = atomicAdd(&sh.n_list, 1);
+                    if (at < BS_LIST) sh.list[at] = (uint64_t)order32(x[i]) << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
                 }
         }
     __syncthreads();
-    int n = n_list;
+    int n = sh.n_list;
     if (n > BS_LIST) {           // too many reach it: the k-th largest value itself, and of its equals the first
         uint32_t lo = order32(bound), top = order32(m);
         while (lo < top) {
@@ -279,51 +279,60 @@ __global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a)
             int c = 0;
 #pragma unroll
             for (int i = 0; i < EPT; i++) c += order32(x[i]) >= at;
-            if (block_total(c, part) >= a.k) lo = at;
+            if (block_total(c, sh.part) >= a.k) lo = at;
             else top = at - 1;
         }
         int above = 0;
 #pragma unroll
         for (int i = 0; i < EPT; i++) above += order32(x[i]) > lo;
-        const int want = a.k - block_total(above, part);
+        const int want = a.k - block_total(above, sh.part);
         int l = first, h = (int)(a.n_vocab - 1 < (int64_t)first + BS_NT * EPT - 1 ? a.n_vocab - 1 : (int64_t)first + BS_NT * EPT - 1);
         while (l < h) {
             const int at = l + (h - l) / 2;
             int c = 0;
 #pragma unroll
             for (int i = 0; i < EPT; i++) c += order32(x[i]) == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= at;
-            if (block_total(c, part) >= want) h = at;
+            if (block_total(c, sh.part) >= want) h = at;
             else l = at + 1;
         }
-        if (tid == 0) n_list = 0;
+        if (tid == 0) sh.n_list = 0;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < EPT; i++) {
             const uint32_t o = order32(x[i]);
-            if (o > lo || (o == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= l)) list[atomicAdd(&n_list, 1)] = (uint64_t)o << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
+            if (o > lo || (o == lo && first + ((i / N) * BS_NT + tid) * N + i % N <= l)) sh.list[atomicAdd(&sh.n_list, 1)] = (uint64_t)o << 32 | (uint32_t)~(first + ((i / N) * BS_NT + tid) * N + i % N);
         }
         __syncthreads();
-        n = n_list;
+        n = sh.n_list;
     }
-    Cand *const out = a.cand + slot * a.k;
     for (int base_i = 0; base_i < n; base_i += BS_NT / 4) {   // four threads a value
         const int i = base_i + (tid >> 2);
-        const uint64_t me = i < n ? list[i] : 0;
+        const uint64_t me = i < n ? sh.list[i] : 0;
         int better = 0;
 #pragma unroll 4
-        for (int j = tid & 3; j < n; j += 4) better += list[j] > me;
+        for (int j = tid & 3; j < n; j += 4) better += sh.list[j] > me;
         better += __shfl_xor_sync(0xffffffffu, better, 1);
         better += __shfl_xor_sync(0xffffffffu, better, 2);
         if (i < n && (tid & 3) == 0 && better < a.k) out[better] = {value32((uint32_t)(me >> 32)), (int)~(uint32_t)me};
     }
     for (int i = n + tid; i < a.k; i += BS_NT) out[i] = {-INFINITY, 0};
     if (tid == BS_NT - 1) {
-        a.top[slot] = m;
+        *out_top = m;
         double t = 0.0;
 #pragma unroll
-        for (int i = 0; i < BS_NT / 32; i++) t += warp_sum[i];
-        a.sum[slot] = t;
+        for (int i = 0; i < BS_NT / 32; i++) t += sh.warp_sum[i];
+        *out_sum = t;
     }
+}
+
+template <typename T, int EPT>
+__global__ void __launch_bounds__(BS_NT, 3) beam_rows_kernel(const SelectArgs a) {
+    pdl_trigger();
+    __shared__ ChunkShared sh;
+    const int64_t row = blockIdx.y, slot = row * a.chunks + blockIdx.x;
+    pdl_wait();
+    if (a.done && a.done[row]) return;       // the merge does not ask for this beam
+    beam_chunk<T, EPT>(a, row, blockIdx.x, a.cand + slot * a.k, a.top + slot, a.sum + slot, sh);
 }
 
 // One candidate of a request: its place among them (beam, chunk, place in the chunk's list) gives the beam
@@ -341,35 +350,36 @@ struct MergeView {
     }
 };
 
-__global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArgs a) {
-    pdl_trigger();
-    __shared__ double offset[BS_MAX_BEAM];   // score of a beam less the logarithm of its sum
-    __shared__ float top_s[BS_MAX_BEAM];
-    __shared__ uint64_t key[BS_LIST];
-    __shared__ int64_t where[BS_LIST];       // beam * vocabulary + token
-    __shared__ uint64_t bound_s, best_s;
-    __shared__ int n_list, part[BS_MERGE_NT / 32];
+struct MergeShared {
+    double offset[BS_MAX_BEAM];              // score of a beam less the logarithm of its sum
+    float top[BS_MAX_BEAM];
+    uint64_t key[BS_LIST];
+    int64_t where[BS_LIST];                  // beam * vocabulary + token
+    uint64_t bound, best;
+    int n_list, part[BS_MERGE_NT / 32];
+};
+
+// Request r of its beams' chunks: candidates, maxima and sums [beam][chunk]
+__device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const Cand *cand, const float *tops, const double *sums, MergeShared &sh) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t r = blockIdx.x, row0 = r * a.n_beam;
+    const int64_t row0 = r * a.n_beam;
     const int per_beam = a.chunks * a.k, total = a.n_beam * per_beam;
-    const Cand *const cand = a.cand + row0 * per_beam;
-    if (tid == 0) n_list = 0;
-    pdl_wait();
+    if (tid == 0) sh.n_list = 0;
     // the first candidates are on their way while the beams' sums are joined
     Cand mine[BS_HELD];
 #pragma unroll
     for (int u = 0; u < BS_HELD; u++) mine[u] = tid + u * BS_MERGE_NT < total ? cand[tid + u * BS_MERGE_NT] : Cand{-INFINITY, 0};
     for (int b = warp; b < a.n_beam; b += BS_MERGE_NT / 32) {
         const int64_t row = row0 + b;
-        float t = lane < a.chunks ? a.top[row * a.chunks + lane] : -INFINITY;   // of an ended beam whatever stands there: not used
-        double part_sum = lane < a.chunks ? a.sum[row * a.chunks + lane] : 0.0;
+        float t = lane < a.chunks ? tops[b * a.chunks + lane] : -INFINITY;   // of an ended beam whatever stands there: not used
+        double part_sum = lane < a.chunks ? sums[b * a.chunks + lane] : 0.0;
         const float score = a.scores[row];
         const bool off = !(score > -INFINITY), ended = a.done && a.done[row];   // off: -inf or NaN
         float m = -INFINITY;
         double s = 0.0;
         if (!ended) {
             m = t;
-            for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, a.top[row * a.chunks + c]);
+            for (int c = lane + 32; c < a.chunks; c += 32) m = fmaxf(m, tops[b * a.chunks + c]);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
             for (int c = lane;;) {
@@ -380,19 +390,19 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
                 }
                 c += 32;
                 if (c >= a.chunks) break;
-                t = a.top[row * a.chunks + c];
-                part_sum = a.sum[row * a.chunks + c];
+                t = tops[b * a.chunks + c];
+                part_sum = sums[b * a.chunks + c];
             }
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         }
         if (lane == 0) {
-            offset[b] = off || (!ended && m == -INFINITY) ? -INFINITY : ended ? (double)score : (double)score - log(s);
-            top_s[b] = ended ? NAN : m;
+            sh.offset[b] = off || (!ended && m == -INFINITY) ? -INFINITY : ended ? (double)score : (double)score - log(s);
+            sh.top[b] = ended ? NAN : m;
         }
     }
     __syncthreads();
-    const MergeView view = {offset, top_s, per_beam};
+    const MergeView view = {sh.offset, sh.top, per_beam};
     uint64_t held[BS_HELD], most = ORDER64_NONE;
 #pragma unroll
     for (int u = 0; u < BS_HELD; u++) {
@@ -418,7 +428,7 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
     };
     auto place = [&](int token, int i) -> int64_t {
         const int b = i / per_beam;
-        return b * a.n_vocab + (top_s[b] != top_s[b] ? a.end_token : token);
+        return b * a.n_vocab + (sh.top[b] != sh.top[b] ? a.end_token : token);
     };
     // Bound: k candidates reach lo.  The k-th largest of the maxima of 32 groups of 16 threads (128 of 4, for k > 32) is one that few more reach; fewer than k groups
     // have any: every candidate passes
@@ -427,59 +437,59 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
         const uint64_t v = __shfl_xor_sync(0xffffffffu, most, o);
         most = v > most ? v : most;
     }
-    if (tid % width == 0) key[tid / width] = most;
+    if (tid % width == 0) sh.key[tid / width] = most;
     __syncthreads();
     {
         int better = 0;   // the threads of a group share the comparisons
 #pragma unroll 2
         for (int j = tid % width; j < groups; j += width) {
-            const uint64_t other = key[j];
+            const uint64_t other = sh.key[j];
             better += other > most || (other == most && j < tid / width);
         }
         for (int o = width / 2; o > 0; o >>= 1) better += __shfl_xor_sync(0xffffffffu, better, o);
-        if (better == a.k - 1) bound_s = most;
-        if (better == 0) best_s = most;
+        if (better == a.k - 1) sh.bound = most;
+        if (better == 0) sh.best = most;
     }
     __syncthreads();
-    uint64_t lo = bound_s > ORDER64_NONE ? bound_s : ORDER64_NONE + 1;
+    uint64_t lo = sh.bound > ORDER64_NONE ? sh.bound : ORDER64_NONE + 1;
     auto list = [&](uint64_t o, int token, int i) {
-        const int e = atomicAdd(&n_list, 1);
+        const int e = atomicAdd(&sh.n_list, 1);
         if (e < BS_LIST) {
-            key[e] = o;
-            where[e] = place(token, i);
+            sh.key[e] = o;
+            sh.where[e] = place(token, i);
         }
         return true;
     };
     count([&](uint64_t o, int token, int i) { return o >= lo && list(o, token, i); });
     __syncthreads();
-    int n = n_list;
+    int n = sh.n_list;
     if (n > BS_LIST) {   // too many reach it: the k-th score itself, and of its equals the first by beam and token
-        uint64_t up = best_s;
+        uint64_t up = sh.best;
         while (lo < up) {
             const uint64_t mid = lo + (up - lo) / 2 + ((up - lo) & 1);
-            if (block_total(count([&](uint64_t o, int, int) { return o >= mid; }), part) >= a.k) lo = mid;
+            if (block_total(count([&](uint64_t o, int, int) { return o >= mid; }), sh.part) >= a.k) lo = mid;
             else up = mid - 1;
         }
-        const int want = a.k - block_total(count([&](uint64_t o, int, int) { return o > lo; }), part);
+        const int want = a.k - block_total(count([&](uint64_t o, int, int) { return o > lo; }), sh.part);
         int64_t l = 0, h = a.n_beam * a.n_vocab - 1;
         while (l < h) {
             const int64_t mid = l + (h - l) / 2;
-            if (block_total(count([&](uint64_t o, int token, int i) { return o == lo && place(token, i) <= mid; }), part) >= want) h = mid;
+            if (block_total(count([&](uint64_t o, int token, int i) { return o == lo && place(token, i) <= mid; }), sh.part) >= want) h = mid;
             else l = mid + 1;
         }
-        if (tid == 0) n_list = 0;
+        if (tid == 0) sh.n_list = 0;
         __syncthreads();
         count([&](uint64_t o, int token, int i) { return (o > lo || (o == lo && place(token, i) <= l)) && list(o, token, i); });
         __syncthreads();
-        n = n_list;
+        n = sh.n_list;
     }
     for (int base_i = 0; base_i < n; base_i += BS_MERGE_NT / 8) {   // eight threads a candidate
         const int i = base_i + (tid >> 3);
-        const uint64_t me = i < n ? key[i] : 0;
-        const int64_t at = i < n ? where[i] : 0;
+        const uint64_t me = i < n ? sh.key[i] : 0;
+        const int64_t at = i < n ? sh.where[i] : 0;
         int better = 0;
 #pragma unroll 2
-        for (int j = tid & 7; j < n; j += 8) better += key[j] > me || (key[j] == me && where[j] < at);
+        for (int j = tid & 7; j < n; j += 8) better += sh.key[j] > me || (sh.key[j] == me && sh.where[j] < at);
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) better += __shfl_xor_sync(0xffffffffu, better, o);
         if (i < n && (tid & 7) == 0 && better < a.k) {
@@ -498,6 +508,37 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
     }
 }
 
+__global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArgs a) {
+    pdl_trigger();
+    __shared__ MergeShared sh;
+    const int64_t r = blockIdx.x, slot0 = r * a.n_beam * a.chunks;
+    pdl_wait();
+    beam_merge(a, r, a.cand + slot0 * a.k, a.top + slot0, a.sum + slot0, sh);
+}
+
+// Both in one launch, for requests of up to 16 chunks in all: a cluster a request.  Every CTA leaves its chunk's candidates in the first one's shared memory, which
+// merges them (4 beams x 32000: 6.5 us of the device in two launches)
+template <typename T, int EPT>
+__global__ void __launch_bounds__(BS_NT) beam_cluster_kernel(const SelectArgs a) {
+    pdl_trigger();
+    __shared__ union {
+        ChunkShared chunk;
+        MergeShared merge;
+    } sh;
+    __shared__ Cand cand[BS_CLUSTER * BS_MAX_K];
+    __shared__ float top[BS_CLUSTER];
+    __shared__ double sum[BS_CLUSTER];
+    const int size = a.n_beam * a.chunks, rank = blockIdx.x % size, beam = rank / a.chunks;
+    const int64_t r = blockIdx.x / size, row = r * a.n_beam + beam;
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");   // the first CTA's shared memory is there
+    pdl_wait();
+    if (!(a.done && a.done[row]))
+        beam_chunk<T, EPT>(a, row, rank - beam * a.chunks, (Cand *)__cluster_map_shared_rank(cand, 0) + rank * a.k, (float *)__cluster_map_shared_rank(top, 0) + rank,
+                           (double *)__cluster_map_shared_rank(sum, 0) + rank, sh.chunk);
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (rank == 0) beam_merge(a, r, cand, top, sum, sh.merge);
+}
+
 // values a thread: 16, or 8 where that would leave SMs without a chunk (and 4 of F32).  (256 threads with 32 values each were 24 warps an SM and waited more:
 // 64 rows of 128256 17.2 us)
 int select_ept(int64_t rows, int64_t n_vocab, int type) {
@@ -507,7 +548,15 @@ int select_ept(int64_t rows, int64_t n_vocab, int type) {
     return least;
 }
 
+// the same for the form with clusters: the fewest values a thread with which a request has no more chunks than that; 0: none
+int select_cluster_ept(int n_beam, int64_t n_vocab, int type) {
+    for (int ept = type == B200_TYPE_F32 ? 4 : 8; ept <= 16; ept *= 2)
+        if (n_beam * ((n_vocab + BS_NT * ept - 1) / (BS_NT * ept)) <= BS_CLUSTER) return ept;
+    return 0;
+}
+
 struct SelectPlan {
+    bool cluster;
     int ept;
     int64_t rows, chunks;
     size_t cand, top, sum, bytes;     // offsets in the workspace
@@ -520,7 +569,9 @@ int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
     B200_REQUIRE(g.k >= 1 && g.k <= BS_MAX_K, "beam_select: %d candidates (1 to %d)", g.k, BS_MAX_K);
     B200_REQUIRE(g.n_vocab >= 1 && g.n_vocab <= (1 << 24) && g.logits_ld >= g.n_vocab, "beam_select: a vocabulary of %lld in rows %lld apart (up to 2^24)", (long long)g.n_vocab, (long long)g.logits_ld);
     p->rows = (int64_t)g.n_request * g.n_beam;
-    p->ept = select_ept(p->rows, g.n_vocab, g.logits_type);
+    p->ept = select_cluster_ept(g.n_beam, g.n_vocab, g.logits_type);
+    p->cluster = p->ept > 0;
+    if (!p->cluster) p->ept = select_ept(p->rows, g.n_vocab, g.logits_type);
     p->chunks = (g.n_vocab + BS_NT * p->ept - 1) / (BS_NT * p->ept);
     B200_REQUIRE(p->rows <= 65535, "beam_select: %lld rows are too many for one launch", (long long)p->rows);
     B200_REQUIRE(p->chunks * g.k * g.n_beam < 0x7fffffffLL, "beam_select: too many candidates of a request");
@@ -532,13 +583,23 @@ int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
     return B200_STATUS_SUCCESS;
 }
 
+template <typename T, int EPT>
+int launch_select(const SelectArgs &a, const SelectPlan &p, int n_request, cudaStream_t s) {
+    if (p.cluster) {
+        const unsigned size = (unsigned)(a.n_beam * a.chunks);
+        if (size > 8) B200_CUDA(cudaFuncSetAttribute(beam_cluster_kernel<T, EPT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        return launch_pdl_cluster(beam_cluster_kernel<T, EPT>, dim3((unsigned)n_request * size), dim3(BS_NT), size, 0, s, a);
+    }
+    const int rc = launch_pdl(beam_rows_kernel<T, EPT>, dim3((unsigned)p.chunks, (unsigned)p.rows), dim3(BS_NT), 0, s, a);
+    if (rc != B200_STATUS_SUCCESS) return rc;
+    return launch_pdl(beam_merge_kernel, dim3((unsigned)n_request), dim3(BS_MERGE_NT), 0, s, a);
+}
 template <typename T>
-int launch_rows(const SelectArgs &a, const SelectPlan &p, cudaStream_t s) {
-    const dim3 grid((unsigned)p.chunks, (unsigned)p.rows);
-    if (p.ept == 16) return launch_pdl(beam_rows_kernel<T, 16>, grid, dim3(BS_NT), 0, s, a);
+int launch_select(const SelectArgs &a, const SelectPlan &p, int n_request, cudaStream_t s) {
+    if (p.ept == 16) return launch_select<T, 16>(a, p, n_request, s);
     if constexpr (sizeof(T) == 4)
-        if (p.ept == 4) return launch_pdl(beam_rows_kernel<T, 4>, grid, dim3(BS_NT), 0, s, a);
-    return launch_pdl(beam_rows_kernel<T, 8>, grid, dim3(BS_NT), 0, s, a);
+        if (p.ept == 4) return launch_select<T, 4>(a, p, n_request, s);
+    return launch_select<T, 8>(a, p, n_request, s);
 }
 
 }  // namespace
@@ -588,11 +649,9 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
     a.out_tokens = g.out_tokens;
     a.out_parents = g.out_parents;
     const cudaStream_t s = (cudaStream_t)stream;
-    if (g.logits_type == B200_TYPE_F32) rc = launch_rows<float>(a, p, s);
-    else if (g.logits_type == B200_TYPE_F16) rc = launch_rows<__half>(a, p, s);
-    else rc = launch_rows<__nv_bfloat16>(a, p, s);
-    if (rc != B200_STATUS_SUCCESS) return rc;
-    return launch_pdl(beam_merge_kernel, dim3((unsigned)g.n_request), dim3(BS_MERGE_NT), 0, s, a);
+    if (g.logits_type == B200_TYPE_F32) return launch_select<float>(a, p, g.n_request, s);
+    if (g.logits_type == B200_TYPE_F16) return launch_select<__half>(a, p, g.n_request, s);
+    return launch_select<__nv_bfloat16>(a, p, g.n_request, s);
 }
 
 }  // extern "C"
