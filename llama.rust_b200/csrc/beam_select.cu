@@ -305,8 +305,8 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs &a, int64_t row, int
         __syncthreads();
         n = sh.n_list;
     }
-    for (int base_i = 0; base_i < n; base_i += BS_NT / 4) {   // four threads a value
-        const int i = base_i + (tid >> 2);
+    for (int at_warp = (tid >> 5) * 8; at_warp < n; at_warp += BS_NT / 4) {   // four threads a value, eight values a warp
+        const int i = at_warp + (lane >> 2);
         const uint64_t me = i < n ? sh.list[i] : 0;
         int better = 0;
 #pragma unroll 4
@@ -483,8 +483,8 @@ __device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const
         __syncthreads();
         n = sh.n_list;
     }
-    for (int base_i = 0; base_i < n; base_i += BS_MERGE_NT / 8) {   // eight threads a candidate
-        const int i = base_i + (tid >> 3);
+    for (int at_warp = warp * 4; at_warp < n; at_warp += BS_MERGE_NT / 8) {   // eight threads a candidate, four candidates a warp
+        const int i = at_warp + (lane >> 3);
         const uint64_t me = i < n ? sh.key[i] : 0;
         const int64_t at = i < n ? sh.where[i] : 0;
         int better = 0;
