@@ -3,13 +3,16 @@
 //
 //   score(b, w) = scores[b] + ((x_w - m) - log sum_v exp(x_v - m)),   m = max_v x_v        (m = +inf: x_w - m is 0 where x_w = m, -inf elsewhere)
 //
-// Bound by reading the logits once.  Two launches:
+// Bound by reading the logits once, but for the latency of what follows the read.  Two launches, or one of clusters for requests of up to 16 chunks:
 //   * beam_rows_kernel: a CTA holds a chunk of a row in registers (512 threads x EPT values), so that maximum, sum of exponentials and the chunk's k best come of
-//     one read.  The k best: the k-th largest of the threads' own maxima is a bound that at least k values reach and few more do; a bisection
-//     over counts (one barrier each) comes near enough to it, the values above are listed and ordered by counting the better ones of each.
-//     Where too many reach the bound (equal values), the bisection goes on over all values, then over the indexes of the equal ones.
+//     one read.  The k best: the k-th largest of the maxima of groups of threads, of which there are 2 k and more, is a bound that at least k values reach and
+//     few more do; those are listed and ordered by counting the better ones of each.  Where more than 512 reach it (equal values), bisections over counts find the k-th value
+//     and, of its equals, the last token.
 //   * beam_merge_kernel: a CTA per request joins the chunks' sums in 64 bits and selects among beams x chunks x k candidates the same way, the scores
-//     in 64 bits: two candidates of different beams are told apart unless their scores agree to about 1e-8.
+//     in 64 bits: two candidates of different beams are told apart unless their scores agree to about 1e-7.
+//   * beam_cluster_kernel: a CTA a chunk leaves its candidates in the first one's shared memory, which merges them.
+// Measured on the device: 64 rows of 128256 F32 (33 MB, 16 candidates) 17 us, 160 of 50001 BF16 15 us, 4 of 32000 F32 6 us.  The chunks' read takes a third of the first; the rest
+// is the latency of barriers and counting, of which an SM overlaps three CTAs.
 // Sums: F32 over a thread's values, 64 bits from there (1e-7 of the sum, so 1e-7 of a score).  The same row gives the same bits wherever it lies:
 // which thread sums which value depends on the vocabulary alone, also where rows do not begin at 16-byte boundaries (their values are then shifted into place).
 #include <cuda_bf16.h>
@@ -63,10 +66,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 constexpr float LOG2E = 1.4426950408889634f, LOWEST = -3.402823466e38f;   // the least finite value
-constexpr uint32_t ORDER32_NONE = 0x007fffffu;               // of -inf
 constexpr uint64_t ORDER64_NONE = 0x000fffffffffffffull;
 
-__device__ __forceinline__ int block_count(bool p) { return __syncthreads_count(p); }
 __device__ __forceinline__ int block_total(int v, int *part) {   // sum over the block; part: one int per warp
     v = __reduce_add_sync(0xffffffffu, v);
     __syncthreads();
@@ -135,8 +136,12 @@ struct Unpack {
     }
 };
 
+// threads of a group of which one maximum is taken: 16, fewer for more candidates
+__device__ __forceinline__ int group_width(int k) { return k <= 16 ? 16 : k <= 32 ? 8 : k <= 64 ? 4 : 2; }
+static_assert(BS_NT >= 4 * BS_MAX_K && BS_MERGE_NT == BS_NT, "two groups of two threads a candidate");
+
 struct ChunkShared {
-    __align__(16) float group_top[32];
+    __align__(16) float group_top[32], small_top[BS_NT / 2];
     float bound;
     double warp_sum[BS_NT / 32];
     uint64_t list[BS_LIST];                  // order of the value, then the complement of the token: larger is better
@@ -199,14 +204,17 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs &a, int64_t row, int
         four[i / 4] = fmaxf(max3(x[i], x[i + 1], x[i + 2]), x[i + 3]);
         mine = fmaxf(mine, four[i / 4]);
     }
-    // maxima of 32 groups of 16 threads, then of the chunk
+    // maxima of 32 groups of 16 threads, then of the chunk; for more than 16 candidates those of smaller groups too
+    const int lane = tid & 31, width = group_width(a.k);
     float g = mine;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    for (int o = 1; o < 16; o <<= 1) {
+        if (o == width && (tid & (width - 1)) == 0) sh.small_top[tid / width] = g;
+        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    }
     if ((tid & 15) == 0) sh.group_top[tid >> 4] = g;
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
-    const int lane = tid & 31;
     const float mine_g = sh.group_top[lane];
     float m = mine_g;
 #pragma unroll
@@ -227,38 +235,28 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs &a, int64_t row, int
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) ds += __shfl_xor_sync(0xffffffffu, ds, o);
     if (lane == 0) sh.warp_sum[tid >> 5] = ds;
-    // A bound that k values of the chunk reach and few more do.  Up to 32 candidates: the k-th largest of the 32 groups' maxima
-    // (of independent values 22 lie above it with k = 16, 130 with 32).  More: bisected over the threads' maxima until few more than k of the 512 have one
-    // (at 192 about 240 values).  It lets every finite value pass where fewer than k maxima are finite
-    float bound;
-    if (a.k <= 32) {
-        // sixteen threads a group, two comparisons each
+    // A bound that k values of the chunk reach and few more do: the k-th largest of the groups' maxima, of which there are 2 k and more (independent values:
+    // at most 1.4 k above it).  A group's threads share the comparisons.  Where fewer than k maxima are finite it lets every finite value pass
+    if (width == 16) {   // (by the loop below: 64 rows of 128256 18.9 us, so 17.2)
         const int j = 2 * (lane & 15), me = tid >> 4;
         const float2 o = *(const float2 *)(sh.group_top + j);
         int better = (o.x > g || (o.x == g && j < me)) + (o.y > g || (o.y == g && j + 1 < me));
 #pragma unroll
         for (int s16 = 8; s16 > 0; s16 >>= 1) better += __shfl_xor_sync(0xffffffffu, better, s16);
         if (better == a.k - 1) sh.bound = g;   // sixteen threads, one value
-        __syncthreads();
-        bound = sh.bound;
     } else {
-        uint32_t lo = ORDER32_NONE + 1, top = order32(m);
-        const uint32_t best = order32(mine);
-        const int enough = 2 * a.k < 192 ? 2 * a.k : 192;
-        if (block_count(best >= lo) > enough)
-            while (lo < top) {
-                const uint32_t at = lo + (top - lo + 1) / 2;
-                const int c = block_count(best >= at);
-                if (c >= a.k) {
-                    lo = at;
-                    if (c <= enough) break;
-                } else {
-                    top = at - 1;
-                }
-            }
-        bound = value32(lo);
+        const int me = tid / width;
+        const float own = sh.small_top[me];
+        int better = 0;
+        for (int j = tid & (width - 1); j < BS_NT / width; j += width) {
+            const float other = sh.small_top[j];
+            better += other > own || (other == own && j < me);
+        }
+        for (int o = width / 2; o > 0; o >>= 1) better += __shfl_xor_sync(0xffffffffu, better, o);
+        if (better == a.k - 1) sh.bound = own;
     }
-    bound = fmaxf(bound, LOWEST);
+    __syncthreads();
+    const float bound = fmaxf(sh.bound, LOWEST);
     // (hits counted by warp and stored without the additions' answers: more instructions, slower)
 #pragma unroll
     for (int f = 0; f < EPT / 4; f++)
@@ -430,9 +428,8 @@ __device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const
         const int b = i / per_beam;
         return b * a.n_vocab + (sh.top[b] != sh.top[b] ? a.end_token : token);
     };
-    // Bound: k candidates reach lo.  The k-th largest of the maxima of 32 groups of 16 threads (128 of 4, for k > 32) is one that few more reach; fewer than k groups
-    // have any: every candidate passes
-    const int groups = a.k <= 32 ? 32 : 128, width = BS_MERGE_NT / groups;
+    // Bound: k candidates reach lo, as above.  Fewer than k groups have any: every candidate passes
+    const int width = group_width(a.k), groups = BS_MERGE_NT / width;
     for (int o = width / 2; o > 0; o >>= 1) {
         const uint64_t v = __shfl_xor_sync(0xffffffffu, most, o);
         most = v > most ? v : most;
@@ -517,7 +514,7 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
 }
 
 // Both in one launch, for requests of up to 16 chunks in all: a cluster a request.  Every CTA leaves its chunk's candidates in the first one's shared memory, which
-// merges them (4 beams x 32000: 6.5 us of the device in two launches)
+// merges them (4 beams x 32000: 6.0 us of the device, 6.5 in two launches, and 2 us less of the host)
 template <typename T, int EPT>
 __global__ void __launch_bounds__(BS_NT) beam_cluster_kernel(const SelectArgs a) {
     pdl_trigger();
@@ -540,7 +537,7 @@ __global__ void __launch_bounds__(BS_NT) beam_cluster_kernel(const SelectArgs a)
 }
 
 // values a thread: 16, or 8 where that would leave SMs without a chunk (and 4 of F32).  (256 threads with 32 values each were 24 warps an SM and waited more:
-// 64 rows of 128256 17.2 us)
+// 64 rows of 128256 17.2 us then, 16.7 so)
 int select_ept(int64_t rows, int64_t n_vocab, int type) {
     const int sms = sm_count(), least = type == B200_TYPE_F32 ? 4 : 8;
     for (int ept = 16; ept > least; ept /= 2)
