@@ -154,6 +154,47 @@ def test_scores_that_grow_along_the_positions(p, n, each):
         pr.run()
 
 
+# One part holds all tiles where the sizes that shape the launch say that there is one: then a tile meets the maximum of those before it
+def one_part(n):
+    return dict(max_len=1000, max_shared=128, max_group=n)
+
+
+@pytest.mark.parametrize("n,each", [(8, 4), (16, 4), (30, 4), (60, 4)])
+@pytest.mark.parametrize("dev", [0.02, 0.3, 4.0])
+def test_scores_that_grow_along_the_positions_of_one_part(p, n, each, dev):
+    pr = Problem(p, [n], [900] * n, [896] * n, "BF16", 64, 1, each, 128)
+    page, place = np.array([P.cell(pr.tables.tolist(), 0, x, 128, pr.n_pages) for x in range(896)]).T
+    pr.q[:, :, 0] = 1.0
+    pr.k[page, place, 0, 0] = P.rounded(np.arange(896) * dev, "BF16")
+    pr.run(one_part(n))
+
+
+@pytest.mark.parametrize("n", [7, 14, 30, 60])
+@pytest.mark.parametrize("ty,value", [("BF16", 9.0), ("BF16", 89.0), ("F16", 95.0), ("BF16", 200.0), ("F16", 300.0), ("BF16", 3000.0)])
+def test_one_position_far_above_the_tiles_before(p, n, ty, value):
+    for at in list(range(512, 528)) + [639, 895]:
+        pr = Problem(p, [n], [900] * n, [896] * n, ty, 64, 1, 4, 128, scale=1.0)
+        page, place = P.cell(pr.tables.tolist(), 0, at, 128, pr.n_pages)
+        pr.q[:] = 0.0
+        pr.q[:, :, 0] = 1.0
+        pr.k[..., 0] *= 0.125
+        pr.k[page, place, 0, 0] = value
+        pr.run(one_part(n))
+
+
+@pytest.mark.parametrize("n", [7, 14, 30, 60])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_one_score_that_is_no_number(p, n, value):
+    for at in list(range(512, 528)) + [3, 895]:
+        pr = Problem(p, [n], [900] * n, [896] * n, "BF16", 64, 1, 4, 128)
+        page, place = P.cell(pr.tables.tolist(), 0, at, 128, pr.n_pages)
+        pr.q[:, :, 0] = 1.0
+        pr.k[page, place, 0, 0] = value
+        pr.call(one_part(n))(None)
+        assert np.isnan(pr.result()).all(), at
+        assert b200.load().kernel_error() == 0
+
+
 def test_a_few_positions_outweigh_all_others(p):
     for at in (0, 127, 128, 500, 767):
         pr = Problem(p, [9], [800] * 9, [768] * 9, "F16", 128, 2, 4, 64)
