@@ -59,29 +59,6 @@ __device__ __forceinline__ void tc_tma(uint32_t dst, const CUtensorMap *map, int
                  : "memory");
 }
 
-// Two powers of two.  Of the exponentials three in eight are computed by multiply-adds, so that the special function units (16 a clock and SM, 1024 clocks a
-// tile) and the others are done at about the same time: y = n + r with |r| <= 1/2, the polynomial is the relative minimax one of 2^r of degree 4 (by
-// Remez' exchange, 2.7e-6), n goes into the exponent.  Below 2^-126 it stays there; above 2^127 (and of a NaN) the result means nothing, which *most, the largest y, tells.
-__device__ __forceinline__ float2 tc_ex2_units(uint64_t y) {
-    const float2 x = pa_split(y);
-    return make_float2(pa_ex2(x.x), pa_ex2(x.y));
-}
-__device__ __forceinline__ float2 tc_ex2_pair(uint64_t y, float *most) {
-    float2 x = pa_split(y);
-    asm("max.NaN.f32 %0, %0, %1, %2;" : "+f"(*most) : "f"(x.x), "f"(x.y));
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
-    const uint64_t v = pa_pair(x.x, x.y), big = pa_pair(12582912.0f, 12582912.0f), neg = pa_pair(-1.0f, -1.0f);   // 1.5 * 2^23: the sum's last bit is 1
-    const uint64_t t = pa_add2(v, big), r = pa_fma2(pa_add2(t, pa_pair(-12582912.0f, -12582912.0f)), neg, v);
-    uint64_t q = pa_pair(9.570102015e-03f, 9.570102015e-03f);
-    q = pa_fma2(q, r, pa_pair(5.591786031e-02f, 5.591786031e-02f));
-    q = pa_fma2(q, r, pa_pair(2.402474482e-01f, 2.402474482e-01f));
-    q = pa_fma2(q, r, pa_pair(6.931218147e-01f, 6.931218147e-01f));
-    q = pa_fma2(q, r, pa_pair(9.999992614e-01f, 9.999992614e-01f));
-    const float2 f = pa_split(q), n = pa_split(t);
-    return make_float2(__uint_as_float(__float_as_uint(f.x) + (__float_as_uint(n.x) << 23)), __uint_as_float(__float_as_uint(f.y) + (__float_as_uint(n.y) << 23)));
-}
-
 __device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t *r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
                  "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
@@ -323,19 +300,19 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                         }
                     }
                     uint64_t ps[2] = {0, 0};   // two running sums each
-                    float most = -INFINITY;
                     const float sub = m == -INFINITY ? 0.0f : -m;
                     const uint64_t sc2 = pa_pair(sc, sc), sub2 = pa_pair(sub, sub);
 #pragma unroll
                     for (int c = 0; c < COLS / 2; c++) {
                         const uint64_t y = pa_fma2(pa_pair(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), sc2, sub2);
-                        const float2 e = (c * 3) % 8 < 3 ? tc_ex2_pair(y, &most) : tc_ex2_units(y);
-                        p[c] = paged_pack<T>(e.x, e.y);
-                        ps[c & 1] = pa_add2(ps[c & 1], pa_pair(e.x, e.y));
+                        // (three in eight by multiply-adds, a polynomial of degree 4, were no faster: 16 a clock and SM are not what a tile waits for)
+                        const float2 x = pa_split(y);
+                        const float e0 = pa_ex2(x.x), e1 = pa_ex2(x.y);
+                        p[c] = paged_pack<T>(e0, e1);
+                        ps[c & 1] = pa_add2(ps[c & 1], pa_pair(e0, e1));
                     }
                     const float2 p0 = pa_split(ps[0]), p1 = pa_split(ps[1]);
-                    float sum = (p0.x + p1.x) + (p0.y + p1.y);
-                    if (!(most < 64.0f)) sum = most + INFINITY;   // far too much, or NaN
+                    const float sum = (p0.x + p1.x) + (p0.y + p1.y);
                     if (anew || !__any_sync(0xffffffffu, sees && !(sum <= TC_MOST))) {
                         if (sees && m > -INFINITY) l += sum;
                         else if (sees && sum != sum) l = sum;   // NaN scores alone
