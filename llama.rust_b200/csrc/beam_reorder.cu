@@ -130,8 +130,12 @@ extern "C" int b200_beam_reorder(const struct b200_beam_reorder_args *args, void
         for (int i = 0; i < 3; i++)
             B200_REQUIRE(!overlap(in[i], in_bytes[i], out[o], out_bytes[o]) && (i >= o || !overlap(out[i], out_bytes[i], out[o], out_bytes[o])), "beam_reorder: an output overlaps another operand");
     for (int i = 0; i < g.n_pools; i++) B200_REQUIRE(g.pools[i] != nullptr && (uintptr_t)g.pools[i] % 16 == 0, "beam_reorder: pool %d is null or not 16-byte aligned", i);
-    int rc = paged_check_device(g.tables_out, "beam_reorder", "tables_out");
-    if (rc == B200_STATUS_SUCCESS && g.n_pools > 0) rc = paged_check_device(g.pools[0], "beam_reorder", "a pool");
+    const PagedOperand mem[6] = {{g.parents, "parents"}, {g.tables_in, "tables_in"}, {g.tables_out, "tables_out"}, {g.lens_in, "lens_in"}, {g.lens_out, "lens_out"}, {g.row_of, "row_of"}};
+    int rc = paged_check_device(mem, 6, "beam_reorder");
+    for (int i = 0; i < g.n_pools && rc == B200_STATUS_SUCCESS; i++) {
+        const PagedOperand pool = {g.pools[i], "a pool"};
+        rc = paged_check_device(&pool, 1, "beam_reorder");
+    }
     if (rc != B200_STATUS_SUCCESS) return rc;
     ReorderArgs a;
     if ((rc = device_error_word(&a.err)) != B200_STATUS_SUCCESS) return rc;

@@ -625,8 +625,9 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
     B200_REQUIRE((uintptr_t)g.logits % size == 0, "beam_select: logits must be aligned to their type");
     B200_REQUIRE(g.workspace != nullptr && (uintptr_t)g.workspace % 256 == 0 && g.workspace_nbytes >= p.bytes, "beam_select: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", p.bytes,
                  g.workspace_nbytes);
-    if ((rc = paged_check_device(g.logits, "beam_select", "logits")) != B200_STATUS_SUCCESS) return rc;
-    if ((rc = paged_check_device(g.workspace, "beam_select", "the workspace")) != B200_STATUS_SUCCESS) return rc;
+    const PagedOperand mem[7] = {{g.logits, "logits"}, {g.scores, "scores"}, {g.done, "done"}, {g.out_scores, "out_scores"}, {g.out_tokens, "out_tokens"}, {g.out_parents, "out_parents"},
+                                 {g.workspace, "the workspace"}};
+    if ((rc = paged_check_device(mem, 7, "beam_select")) != B200_STATUS_SUCCESS) return rc;
     uint8_t *const ws = (uint8_t *)g.workspace;
     SelectArgs a;
     a.logits = (const uint8_t *)g.logits;

@@ -19,8 +19,12 @@ struct PagedCache {
 };
 
 int paged_check_cache(const b200_paged_cache &c, const char *op, PagedCache *out);   // paged_append.cu
-// refuses memory that no kernel of the current device may touch: another device's, or the host's pageable memory
-int paged_check_device(const void *p, const char *op, const char *what);
+// refuses operands (null: not given) that no kernel of the current device may touch: another device's memory, the host's pageable memory
+struct PagedOperand {
+    const void *p;
+    const char *name;
+};
+int paged_check_device(const PagedOperand *operands, int n, const char *op);
 
 // Byte offset of position p of sequence s in the cache (K and V alike), or -1 where the table or a page id does not reach
 __device__ __forceinline__ int64_t paged_row(const PagedCache &c, int s, int p) {

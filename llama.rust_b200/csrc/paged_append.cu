@@ -12,16 +12,20 @@
 
 namespace b200 {
 
-int paged_check_device(const void *p, const char *op, const char *what) {
-    cudaPointerAttributes at;
+int paged_check_device(const PagedOperand *operands, int n, const char *op) {
     int dev = 0;
     B200_CUDA(cudaGetDevice(&dev));
-    if (cudaPointerGetAttributes(&at, p) != cudaSuccess) {
-        cudaGetLastError();
-        B200_REQUIRE(false, "%s: %s is not memory that a kernel can touch", op, what);
+    for (int i = 0; i < n; i++) {
+        const char *const what = operands[i].name;
+        if (operands[i].p == nullptr) continue;
+        cudaPointerAttributes at;
+        if (cudaPointerGetAttributes(&at, operands[i].p) != cudaSuccess) {
+            cudaGetLastError();
+            B200_REQUIRE(false, "%s: %s is not memory that a kernel can touch", op, what);
+        }
+        B200_REQUIRE(at.type != cudaMemoryTypeUnregistered, "%s: %s is pageable host memory", op, what);
+        B200_REQUIRE(at.type != cudaMemoryTypeDevice || at.device == dev, "%s: %s is memory of device %d, the current device is %d", op, what, at.device, dev);
     }
-    B200_REQUIRE(at.type != cudaMemoryTypeUnregistered, "%s: %s is pageable host memory", op, what);
-    B200_REQUIRE(at.type != cudaMemoryTypeDevice || at.device == dev, "%s: %s is memory of device %d, the current device is %d", op, what, at.device, dev);
     return B200_STATUS_SUCCESS;
 }
 
@@ -195,10 +199,9 @@ extern "C" int b200_paged_append(const struct b200_paged_append_args *args, void
     if (g.n_head) all |= (uintptr_t)g.q;
     const uint64_t out = g.n_head ? (uintptr_t)g.q_out | (uint64_t)nb[6] | (uint64_t)nb[7] : 0;
     B200_REQUIRE(all % xs == 0 && out % 2 == 0, "paged_append: rows and strides must be aligned to their elements");
-    const void *mem[3] = {g.cache.k, g.k, g.n_head ? g.q_out : g.cache.v};
-    const char *names[3] = {"the cache", "k", "q_out"};
-    for (int i = 0; i < 3; i++)
-        if ((rc = paged_check_device(mem[i], "paged_append", names[i])) != B200_STATUS_SUCCESS) return rc;
+    const PagedOperand mem[10] = {{g.cache.k, "the cache's keys"}, {g.cache.v, "the cache's values"}, {g.cache.tables, "tables"}, {g.pos, "pos"}, {g.seq, "seq"},
+                                  {g.k, "k"}, {g.v, "v"}, {g.n_head ? g.q : nullptr, "q"}, {g.n_head ? g.q_out : nullptr, "q_out"}, {g.n_dims ? g.rope : nullptr, "rope"}};
+    if ((rc = paged_check_device(mem, 10, "paged_append")) != B200_STATUS_SUCCESS) return rc;
     a.n_tok = g.n_tok;
     a.pos = g.pos;
     a.seq = g.seq;

@@ -210,3 +210,35 @@ def test_host_memory_is_refused(p):
         with pytest.raises(Exception, match="host memory|kernel can touch"):
             call(None)
     torch.cuda.synchronize()
+
+
+def test_every_operand_in_host_memory_is_refused(p):
+    import torch
+    host = np.zeros(1 << 20, dtype=np.uint8)
+    base = (host.ctypes.data + 255) // 256 * 256
+    room = torch.zeros(1 << 20, dtype=torch.uint8, device="cuda")
+    at = [room.data_ptr() + (i << 16) for i in range(16)]
+    c = p.Cache(p.BF16, 16, 4, 2, 64, at[0], at[1], at[2], 4, 2)
+    calls = (p.Append(c, 2, p.F32, at[3], at[4], at[5], seq=at[6], q=at[7], q_out=at[8], n_head=4, rope=at[9], rope_rows=8, rope_ld=64, n_dims=64),
+             p.PrefixAttn(c, 2, 4, at[3], at[4], at[5], 0.1, shared=at[6], group_first=at[7], n_group=1, sinks=at[8], max_len=40, max_shared=32, max_group=2),
+             p.BeamSelect(p.F32, 1, 2, 1000, 2, at[3], at[4], at[5], at[6], at[7], done=at[8]),
+             p.BeamReorder(1, 2, at[3], at[4], at[5], 4, at[6], at[7], at[8], 16, 4, 64, [at[9], at[10]]))
+    refused = 0
+    for call in calls:
+        call(None)   # as it stands it runs
+        for args in (call.args, getattr(call.args, "cache", None)):
+            for name, ty in (args._fields_ if args is not None else ()):
+                if ty is not p.vp:
+                    continue
+                kept = getattr(args, name)
+                setattr(args, name, base)
+                with pytest.raises(Exception, match="host memory|kernel can touch"):
+                    call(None)
+                setattr(args, name, kept)
+                refused += 1
+    calls[3].pools[1] = base
+    with pytest.raises(Exception, match="host memory|kernel can touch"):
+        calls[3](None)
+    torch.cuda.synchronize()
+    # groups of zeros: [0, 0) holds none of the two sequences, which attention reports
+    assert refused == 7 + 3 + 7 + 3 + 7 + 6 and b200.load().kernel_error() == 7
