@@ -41,7 +41,7 @@ struct b200_paged_cache {
  * channels of a head rotate, in pairs (2 i, 2 i + 1) (mode 0, NORMAL) or (i, i + n_dims / 2) (mode 2, NEOX); the others are copied.  rope: (cos, sin)
  * rows by position as b200_rope_table makes them (pair i of a row at 2 i and 2 i + 1), rope_ld floats apart.  Strides are bytes per
  * token and per head.  Queries (n_head 0: none) go to q_out in the cache's type; q_out may be q where types and strides are the same.  Two tokens
- * of one call at the same position of a sequence: one of them is stored, per 16 channels; which is not said. */
+ * of one call at the same position of a sequence: what stands there afterwards is channels of either. */
 struct b200_paged_append_args {
     struct b200_paged_cache cache;
     int64_t n_tok;

@@ -201,7 +201,7 @@ int prefix_plan(const b200_prefix_attn_args &g, PrefixPlan *p) {
     p->rows = (int64_t)g.n_seq * g.n_head;
     // one sequence shares nothing, and less than a tile is no shared part
     const int64_t shared_tiles = g.n_group && g.max_group > 1 ? g.max_shared / PX_TILE : 0;
-    a.served = shared_tiles > 0 ? g.max_group : 0;
+    a.served = shared_tiles > 0 ? (int)(g.max_group < g.n_seq ? g.max_group : g.n_seq) : 0;
     a.shared_blocks = 0;
     const int64_t shared_rows = (int64_t)a.served * a.each, block_rows = prefix_shared_rows(shared_rows);
     if (a.served) {

@@ -264,6 +264,10 @@ def test_sizes_that_shape_the_launch_are_hints(p, hints):
     Problem(p, [], [700, 1, 333], [0] * 3, "F16", 128, 2, 4).run(hints)
 
 
+def test_sizes_that_shape_the_launch_may_be_the_largest(p):
+    Problem(p, [5, 2], [300, 280, 257, 256, 600, 40, 33], [256, 256, 256, 256, 256, 32, 32], "BF16", 64, 2, 2, 16).run(dict(max_len=2 ** 31 - 1, max_shared=2 ** 31 - 1, max_group=2 ** 31 - 1))
+
+
 def test_wide_scores_and_a_negative_scale(p):
     Problem(p, [6], [500] * 6, [450] * 6, "F16", 128, dev=4.0).run()
     Problem(p, [6], [500] * 6, [450] * 6, "F16", 64, scale=-0.3).run()

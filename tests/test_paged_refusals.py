@@ -119,3 +119,11 @@ def test_workspaces_hold_every_part(p):
     s = p.lib.b200_beam_select_workspace_nbytes
     assert s(C.byref(select_of(p, n_vocab=128256).args)) > s(C.byref(select_of(p).args)) >= 8 * 8 * 8
     assert s(C.byref(select_of(p, k=0).args)) == 0
+
+
+def test_sizes_that_shape_the_launch_may_be_anything(p):
+    most = 2 ** 31 - 1
+    import ctypes
+    for kw in (dict(max_group=most, max_shared=most, max_len=most), dict(max_group=most), dict(max_shared=most), dict(max_len=most), dict(max_group=0, max_shared=0, max_len=0)):
+        call = attn_of(p, **kw)
+        assert p.lib.b200_prefix_attn_workspace_nbytes(ctypes.byref(call.args)) > 0, kw
