@@ -64,7 +64,7 @@ struct alignas(128) PxUnit {                  // shared memory of four warps
 };
 
 // Four warps walk the items unit, unit + n_units, ..: a stream of tiles of 64 positions, PX_STAGES ahead of the products, whichever items they belong to, so
-// that an item costs little besides its tiles (item by item, its look-ups, queries and first tile in front of each, took twice the time on four tiles).  Warp w has positions 16 w .. + 15 of
+// that an item costs little besides its tiles (item by item, its look-ups, queries and first tile in front of each, took twice the time on four tiles; items handed to a CTA's units as they come to them were no faster).  Warp w has positions 16 w .. + 15 of
 // every tile, its own maximum and sum, and leaves a part of its own for the merge.  Positions that the sequence does not see are zeros in shared memory,
 // whatever the page holds.  tid: 0 .. 127; barrier: a named one of these four warps
 template <typename T, int D>
