@@ -77,6 +77,20 @@ def test_a_large_vocabulary(p):
     select(p, head(rng, 1, 2, 1000003, "F16"), -rng.random((1, 2)), 4, "F16")
 
 
+@pytest.mark.parametrize("k", [15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128])
+@pytest.mark.parametrize("B,V", [(2, 9001), (9, 20000)])
+def test_where_the_best_logits_lie(p, k, B, V):
+    # spread out; side by side, so that one thread's and one group's values are the best; few that are finite
+    rng = np.random.default_rng(k)
+    x = head(rng, 2, B, V)
+    select(p, x, -rng.random((2, B)), k)
+    side = np.sort(x, axis=-1)
+    select(p, side, -rng.random((2, B)), k)
+    few = np.full_like(x, -np.inf)
+    few[..., ::V // 20] = x[..., ::V // 20]
+    select(p, few, -rng.random((2, B)), k)
+
+
 @pytest.mark.parametrize("offset", [0.0, 30.0, -500.0, 2000.0])
 def test_logits_far_from_zero(p, offset):
     # x log2(e) is rounded once for a chunk's maximum: what that is off by must not show
