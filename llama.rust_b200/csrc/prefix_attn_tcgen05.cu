@@ -8,7 +8,7 @@
 //   * K and V come in tiles of 128 positions by TMA, a box a page (or as much of a page as a tile holds), the pages' ids read a tile ahead; K is a K-major
 //     and V an MN-major B operand, so neither is transposed.  A page id out of range is loaded from behind the last page (zeros), and the part's rows are marked to be
 //     computed again without it.
-//   * Two groups of four softmax warps work in turn (as published with FlashAttention-4): with one block of rows they take the tiles alternately, each with
+//   * Two groups of four softmax warps work in turn: with one block of rows they take the tiles alternately, each with
 //     an output of its own; with two blocks each has its block and both read every tile.  While one computes weights the tensor cores have the other's
 //     products.  A thread owns a row; weights go back into tensor memory over the scores they came from, as the A operand of the second product.
 //   * A row sees a tile as a whole or not at all, so that no score is masked one by one.
