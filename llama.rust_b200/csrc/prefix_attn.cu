@@ -2,14 +2,14 @@
 //
 //   o = sum_p w_p v_p / (sum_p w_p + exp(sink)),  w_p = exp(scale q k_p - max)          softmax in one pass, running maximum and sum in F32
 //
-// Rows that share positions share key heads too.  prefix_shared_kernel (prefix_attn_tcgen05.cu) takes the whole tiles of 128 positions that a sequence shares, all rows
+// Rows that share positions share key heads too.  The shared part (prefix_attn_tcgen05.cu) takes the whole tiles of 128 positions that a sequence shares, all rows
 // of a group and key head together; the own part (prefix_attn_own.cuh) what is left of a sequence, the query heads of a key head together.  Either cuts its positions
 // into parts that leave (accumulator, maximum, sum) in the workspace; one launch has the CTAs of both, prefix_merge_kernel joins a row's parts, a warp each.
 // Measured on the device, 32 heads on 8 of 128, BF16 (other where it says so), of the bytes that each cached position costs once at the copy rate:
 //   a group of 64 rows, 32768 shared positions, up to 512 of a row's own     60.6 us, 252 MB: 4.2 TB/s, 0.64; 34.3 GFLOP: 566 TFLOP/s
-//   4 groups of 16 rows, 4096 shared, up to 128 own                         25.8 us, 97 MB: 3.8 TB/s, 0.58
-//   3 groups of 7 rows, 2047 shared, up to 333 own, F16, 16 key heads of 64 22 us, 49 MB: 2.2 TB/s, 0.35
-//   a group of 8 rows, 1000 shared, up to 24 own, F16                       9.6 us, of which the second launch 4.6
+//   4 groups of 16 rows, 4096 shared, up to 128 own                         24.6 us, 97 MB: 4.0 TB/s, 0.61
+//   3 groups of 7 rows, 2047 shared, up to 333 own, F16, 16 key heads of 64 21 us, 49 MB: 2.3 TB/s, 0.36
+//   a group of 8 rows, 1000 shared, up to 24 own, F16                       9.5 us, of which the second launch 4.6
 // Above a few thousand positions the chain of a tile bounds it (scores, weights, products: prefix_attn_tcgen05.cu), below that beginnings and ends: 5 us of a CTA, the
 // second launch.
 #include <cmath>

@@ -86,6 +86,19 @@ __device__ __forceinline__ void prefix_own_stream(const PrefixArgs &a, int unit,
     // an item's length and shared positions are read an item ahead
     int ahead_len = 0, ahead_shared = 0, grp_first = 0, grp_end = 0;   // the group of the item before: most likely this one's too
     bool in_group = false;
+    // up to 32 groups are looked through in registers (two trips to memory an item otherwise, 1 us)
+    const int my_first = lane < a.n_group ? a.group_first[lane] : 0, my_end = lane < a.n_group ? a.group_first[lane + 1] : 0;
+    auto find_group = [&](int s) -> bool {
+        if (a.n_group == 0 || a.n_group > 32) return prefix_group(a, s, &grp_first, &grp_end);
+        const int g = 31 - __clz(__ballot_sync(0xffffffffu, lane < a.n_group && my_first <= s) | 1u);
+        grp_first = __shfl_sync(0xffffffffu, my_first, g);
+        grp_end = __shfl_sync(0xffffffffu, my_end, g);
+        if (prefix_group_fits(grp_first, grp_end, a.n_seq) && s >= grp_first && s < grp_end) return true;
+        if (lane == 0) atomicExch(a.err, ERR_PAGED);
+        grp_first = s;
+        grp_end = s + 1;
+        return false;
+    };
     auto read_ahead = [&](int item) {
         if (item < n_items) {
             ahead_len = a.lens[item / of_seq];
@@ -107,7 +120,7 @@ __device__ __forceinline__ void prefix_own_stream(const PrefixArgs &a, int unit,
             const int len = ahead_len;
             it.shared = ahead_shared;
             read_ahead(next_item + n_units);
-            if (it.s < grp_first || it.s >= grp_end) in_group = prefix_group(a, it.s, &grp_first, &grp_end);
+            if (it.s < grp_first || it.s >= grp_end) in_group = find_group(it.s);
             it.first = grp_first;
             const bool served = in_group && it.s - grp_first < a.served;
             if (len > capacity && tid == 0) atomicExch(a.err, ERR_PAGED);
