@@ -66,6 +66,9 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return r;
 }
 constexpr float LOG2E = 1.4426950408889634f, LOWEST = -3.402823466e38f;   // the least finite value
+// Maxima up to which a chunk's exponentials are one multiply-add each, exp2(x log2(e) - c) with c = m log2(e) rounded: c is then below 2^13, off by 2^-12 at most, and
+// what the merge's first-order correction leaves, (ln 2 2^-12)^2 / 2 = 1.4e-8, is less than half a step of F32.  Above it m is subtracted first
+constexpr float NEAR_ZERO = 4096.0f;
 constexpr uint64_t ORDER64_NONE = 0x000fffffffffffffull;
 
 __device__ __forceinline__ int block_total(int v, int *part) {   // sum over the block; part: one int per warp
@@ -219,9 +222,9 @@ __device__ __forceinline__ void beam_chunk(const SelectArgs &a, int64_t row, int
     float m = mine_g;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    // sum of exponentials: exp2(x log2(e) - c) with c = m log2(e) rounded, one multiply-add each; what the rounding of c is off by, the merge puts right
+    // sum of exponentials; what the rounding of c is off by, the merge puts right
     float s = 0.0f;
-    if (fabsf(m) < 1e30f) {
+    if (fabsf(m) <= NEAR_ZERO) {
         const float c = m * LOG2E;
         float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -383,7 +386,7 @@ __device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const
             for (int c = lane;;) {
                 // exp(t - m), and what c = t log2(e) was off by when the chunk's exponentials were taken
                 if (t > -INFINITY) {
-                    const double back = fabsf(t) < 1e30f ? 1.0 - 0.6931471805599453 * (double)fmaf(t, LOG2E, -(t * LOG2E)) : 1.0;
+                    const double back = fabsf(t) <= NEAR_ZERO ? 1.0 - 0.6931471805599453 * (double)fmaf(t, LOG2E, -(t * LOG2E)) : 1.0;
                     s += part_sum * back * (t == m ? 1.0 : fabsf(m) < 1e30f ? (double)fast_exp2((t - m) * LOG2E) : exp((double)t - (double)m));
                 }
                 c += 32;
