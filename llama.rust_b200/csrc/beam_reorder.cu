@@ -104,8 +104,6 @@ __global__ void __launch_bounds__(BR_NT) beam_reorder_kernel(const __grid_consta
     }
 }
 
-bool overlap(const void *a, size_t na, const void *b, size_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
-
 }  // namespace
 }  // namespace b200
 
@@ -129,7 +127,7 @@ extern "C" int b200_beam_reorder(const struct b200_beam_reorder_args *args, void
     const size_t in_bytes[3] = {ids, tables, ids}, out_bytes[3] = {tables, ids, g.row_of ? ids : 0};
     for (int o = 0; o < 3; o++)
         for (int i = 0; i < 3; i++)
-            B200_REQUIRE(!overlap(in[i], in_bytes[i], out[o], out_bytes[o]) && (i >= o || !overlap(out[i], out_bytes[i], out[o], out_bytes[o])), "beam_reorder: an output overlaps another operand");
+            B200_REQUIRE(!paged_overlap(in[i], in_bytes[i], out[o], out_bytes[o]) && (i >= o || !paged_overlap(out[i], out_bytes[i], out[o], out_bytes[o])), "beam_reorder: an output overlaps another operand");
     for (int i = 0; i < g.n_pools; i++) B200_REQUIRE(g.pools[i] != nullptr && (uintptr_t)g.pools[i] % 16 == 0, "beam_reorder: pool %d is null or not 16-byte aligned", i);
     const PagedOperand mem[6] = {{g.parents, "parents"}, {g.tables_in, "tables_in"}, {g.tables_out, "tables_out"}, {g.lens_in, "lens_in"}, {g.lens_out, "lens_out"}, {g.row_of, "row_of"}};
     int rc = paged_check_device(mem, 6, "beam_reorder");

@@ -628,6 +628,16 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
     B200_REQUIRE((uintptr_t)g.logits % size == 0, "beam_select: logits must be aligned to their type");
     B200_REQUIRE(g.workspace != nullptr && (uintptr_t)g.workspace % 256 == 0 && g.workspace_nbytes >= p.bytes, "beam_select: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", p.bytes,
                  g.workspace_nbytes);
+    // A request's scores are read until its choice is made: another's results must not lie on them.  Its own may, where there are as many
+    const size_t rows4 = (size_t)p.rows * 4, outs = (size_t)g.n_request * g.k * 4;
+    const void *const in[3] = {g.logits, g.scores, g.done}, *const out[4] = {g.out_scores, g.out_tokens, g.out_parents, g.workspace};
+    const size_t in_bytes[3] = {(size_t)((p.rows - 1) * g.logits_ld + g.n_vocab) * size, rows4, g.done ? (size_t)p.rows : 0}, out_bytes[4] = {outs, outs, outs, p.bytes};
+    for (int o = 0; o < 4; o++) {
+        for (int i = 0; i < 3; i++)
+            B200_REQUIRE(!paged_overlap(in[i], in_bytes[i], out[o], out_bytes[o]) || (i == 1 && o == 0 && g.scores == g.out_scores && g.k == g.n_beam),
+                         "beam_select: an output or the workspace overlaps another operand");
+        for (int i = 0; i < o; i++) B200_REQUIRE(!paged_overlap(out[i], out_bytes[i], out[o], out_bytes[o]), "beam_select: an output or the workspace overlaps another operand");
+    }
     const PagedOperand mem[7] = {{g.logits, "logits"}, {g.scores, "scores"}, {g.done, "done"}, {g.out_scores, "out_scores"}, {g.out_tokens, "out_tokens"}, {g.out_parents, "out_parents"},
                                  {g.workspace, "the workspace"}};
     if ((rc = paged_check_device(mem, 7, "beam_select")) != B200_STATUS_SUCCESS) return rc;

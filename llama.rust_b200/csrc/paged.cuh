@@ -25,6 +25,7 @@ struct PagedOperand {
     const char *name;
 };
 int paged_check_device(const PagedOperand *operands, int n, const char *op);
+inline bool paged_overlap(const void *a, size_t na, const void *b, size_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }
 
 // Byte offset of position p of sequence s in the cache (K and V alike), or -1 where the table or a page id does not reach
 __device__ __forceinline__ int64_t paged_row(const PagedCache &c, int s, int p) {
