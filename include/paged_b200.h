@@ -85,7 +85,7 @@ int b200_prefix_attn(const struct b200_prefix_attn_args *args, void *stream);
 
 /* The k best continuations of every request: candidate (b, w) scores scores[b] + log softmax(logits[b])[w], and a beam that has ended (done[b] != 0)
  * has one candidate, (b, end_token) with scores[b].  They come in descending order of their scores, held in 64 bits until they are stored; equal ones
- * by beam, then by token.  A logit that is NaN or -inf, and a beam whose score is NaN or -inf, has no candidates; several logits of +inf share the
+ * by beam, then by logit, then by token.  A logit that is NaN or -inf, and a beam whose score is NaN or -inf, has no candidates; several logits of +inf share the
  * whole probability.  Where fewer than k candidates are left, the rest are score -inf, token -1, parent -1.  out_scores may be scores where k is n_beam;
  * any other overlap of the outputs or the workspace with an operand is refused. */
 struct b200_beam_select_args {

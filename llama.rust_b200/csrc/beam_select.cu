@@ -1,5 +1,5 @@
 // The k best continuations of a request's beams (b200_beam_select): log softmax over every beam's logits, the beam's score added, and the k
-// best of beams x vocabulary in the order of (score in 64 bits, beam, token).
+// best of beams x vocabulary in the order of (score in 64 bits, beam, logit, token).
 //
 //   score(b, w) = scores[b] + ((x_w - m) - log sum_v exp(x_v - m)),   m = max_v x_v        (m = +inf: x_w - m is 0 where x_w = m, -inf elsewhere)
 //
@@ -355,7 +355,7 @@ struct MergeShared {
     double offset[BS_MAX_BEAM];              // score of a beam less the logarithm of its sum
     float top[BS_MAX_BEAM];
     uint64_t key[BS_LIST];
-    int64_t where[BS_LIST];                  // beam * vocabulary + token
+    uint64_t where[BS_LIST];                 // what comes first among equal scores is less
     uint64_t bound, best;
     int n_list, part[BS_MERGE_NT / 32];
 };
@@ -415,22 +415,21 @@ __device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const
         const uint64_t o = view.order(i, cand[i].value);
         most = o > most ? o : most;
     }
-    // count of a thread's own candidates for which f(order, place) holds
+    // count of a thread's own candidates for which f(order, candidate, place) holds
     auto count = [&](auto f) -> int {
         int c = 0;
 #pragma unroll
-        for (int u = 0; u < BS_HELD; u++) c += held[u] > ORDER64_NONE && f(held[u], mine[u].token, tid + u * BS_MERGE_NT);
+        for (int u = 0; u < BS_HELD; u++) c += held[u] > ORDER64_NONE && f(held[u], mine[u], tid + u * BS_MERGE_NT);
         for (int i = tid + BS_HELD * BS_MERGE_NT; i < total; i += BS_MERGE_NT) {
             const Cand cd = cand[i];
             const uint64_t o = view.order(i, cd.value);
-            c += o > ORDER64_NONE && f(o, cd.token, i);
+            c += o > ORDER64_NONE && f(o, cd, i);
         }
         return c;
     };
-    auto place = [&](int token, int i) -> int64_t {
-        const int b = i / per_beam;
-        return b * a.n_vocab + (sh.top[b] != sh.top[b] ? a.end_token : token);
-    };
+    // beam (6 bits), then the complement of the logit's order (a beam's larger logits come first, also where 64 bits do not tell their scores apart), then token (24
+    // bits; of an ended beam's only candidate logit and token are whatever stands there)
+    auto place = [&](const Cand &cd, int i) -> uint64_t { return (uint64_t)(i / per_beam) << 56 | (uint64_t)~order32(cd.value) << 24 | (cd.token & 0xffffff); };
     // Bound: k candidates reach lo, as above.  Fewer than k groups have any: every candidate passes
     const int width = group_width(a.k), groups = BS_MERGE_NT / width;
     for (int o = width / 2; o > 0; o >>= 1) {
@@ -452,41 +451,41 @@ __device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const
     }
     __syncthreads();
     uint64_t lo = sh.bound > ORDER64_NONE ? sh.bound : ORDER64_NONE + 1;
-    auto list = [&](uint64_t o, int token, int i) {
+    auto list = [&](uint64_t o, const Cand &cd, int i) {
         const int e = atomicAdd(&sh.n_list, 1);
         if (e < BS_LIST) {
             sh.key[e] = o;
-            sh.where[e] = place(token, i);
+            sh.where[e] = place(cd, i);
         }
         return true;
     };
-    count([&](uint64_t o, int token, int i) { return o >= lo && list(o, token, i); });
+    count([&](uint64_t o, const Cand &cd, int i) { return o >= lo && list(o, cd, i); });
     __syncthreads();
     int n = sh.n_list;
-    if (n > BS_LIST) {   // too many reach it: the k-th score itself, and of its equals the first by beam and token
+    if (n > BS_LIST) {   // too many reach it: the k-th score itself, and of its equals the first by beam, logit and token
         uint64_t up = sh.best;
         while (lo < up) {
             const uint64_t mid = lo + (up - lo) / 2 + ((up - lo) & 1);
-            if (block_total(count([&](uint64_t o, int, int) { return o >= mid; }), sh.part) >= a.k) lo = mid;
+            if (block_total(count([&](uint64_t o, const Cand &, int) { return o >= mid; }), sh.part) >= a.k) lo = mid;
             else up = mid - 1;
         }
-        const int want = a.k - block_total(count([&](uint64_t o, int, int) { return o > lo; }), sh.part);
-        int64_t l = 0, h = a.n_beam * a.n_vocab - 1;
+        const int want = a.k - block_total(count([&](uint64_t o, const Cand &, int) { return o > lo; }), sh.part);
+        uint64_t l = 0, h = ((uint64_t)a.n_beam << 56) - 1;
         while (l < h) {
-            const int64_t mid = l + (h - l) / 2;
-            if (block_total(count([&](uint64_t o, int token, int i) { return o == lo && place(token, i) <= mid; }), sh.part) >= want) h = mid;
+            const uint64_t mid = l + (h - l) / 2;
+            if (block_total(count([&](uint64_t o, const Cand &cd, int i) { return o == lo && place(cd, i) <= mid; }), sh.part) >= want) h = mid;
             else l = mid + 1;
         }
         if (tid == 0) sh.n_list = 0;
         __syncthreads();
-        count([&](uint64_t o, int token, int i) { return (o > lo || (o == lo && place(token, i) <= l)) && list(o, token, i); });
+        count([&](uint64_t o, const Cand &cd, int i) { return (o > lo || (o == lo && place(cd, i) <= l)) && list(o, cd, i); });
         __syncthreads();
         n = sh.n_list;
     }
     for (int at_warp = warp * 4; at_warp < n; at_warp += BS_MERGE_NT / 8) {   // eight threads a candidate, four candidates a warp
         const int i = at_warp + (lane >> 3);
         const uint64_t me = i < n ? sh.key[i] : 0;
-        const int64_t at = i < n ? sh.where[i] : 0;
+        const uint64_t at = i < n ? sh.where[i] : 0;
         int better = 0;
 #pragma unroll 2
         for (int j = tid & 7; j < n; j += 8) better += sh.key[j] > me || (sh.key[j] == me && sh.where[j] < at);
@@ -495,10 +494,10 @@ __device__ __forceinline__ void beam_merge(const SelectArgs &a, int64_t r, const
         if (i < n && (tid & 7) == 0 && better < a.k) {
             const int64_t e = r * a.k + better;
             const uint64_t bits = me >> 63 ? me & ~(1ull << 63) : ~me;
-            const int b = (int)(at / a.n_vocab);
             a.out_scores[e] = (float)__longlong_as_double((long long)bits);
+            const int b = (int)(at >> 56);
             a.out_parents[e] = b;
-            a.out_tokens[e] = (int32_t)(at - b * a.n_vocab);
+            a.out_tokens[e] = sh.top[b] != sh.top[b] ? a.end_token : (int32_t)(at & 0xffffff);
         }
     }
     for (int i = n + tid; i < a.k; i += BS_MERGE_NT) {

@@ -3,6 +3,7 @@ maximum is exact where it counts (words within a factor of two of it, or within 
 import numpy as np
 import pytest
 
+import b200
 import plain_paged as P
 from test_gpu_beam import head, p, select  # noqa: F401
 
@@ -59,3 +60,71 @@ def test_the_sum_is_as_good_far_from_zero(p):
         for R, B, V in FORMS:
             x = P.rounded(offset - 8.0 * rng.random((R, B, V)), "F32")
             select(p, x, -rng.random((R, B)), 4)
+
+
+def chosen(p, x, scores, k):
+    """F32 logits [requests, beams, vocab] -> (scores, tokens, parents), held to the definition; scores may be infinite"""
+    m = b200.load()
+    R, B, V = x.shape
+    scores = np.asarray(scores, dtype=np.float32)
+    keep = [m.device_array(np.ascontiguousarray(x, dtype=np.float32)), m.device_array(scores)]
+    outs = [m.device_array(np.full(R * k, 77, dtype=np.int32)) for _ in range(3)]
+    p.BeamSelect(p.F32, R, B, V, k, keep[0].ptr, keep[1].ptr, *(o.ptr for o in outs))(None)
+    s, w, b = (o.download(np.int32, R * k).reshape(R, k) for o in outs)
+    s = s.view(np.float32).astype(np.float64)
+    for r in range(R):
+        found = []
+        for j in range(B):
+            v = x[r, j].astype(np.float32).astype(np.float64)
+            if not scores[r, j] > -np.inf or v.max() == -np.inf:
+                continue
+            with np.errstate(invalid="ignore"):
+                off = np.where(v == v.max(), 0.0, v - v.max())
+                gain = float(scores[r, j]) + (off - np.log(np.exp(off).sum()))
+            best = np.lexsort((np.arange(V), -v, -gain))[:k]   # NaN (none of the words beside one of +inf) comes last
+            found += [(-gain[t], j, -v[t], int(t)) for t in best if gain[t] > -np.inf]
+        found = sorted(found)[:k]
+        n = len(found)
+        assert [(f[1], f[3]) for f in found] == list(zip(b[r, :n].tolist(), w[r, :n].tolist()))
+        want = -np.array([f[0] for f in found])
+        assert ((np.abs(s[r, :n] - want) <= 2.0 ** -23 * np.abs(want) + 2.0 ** -20) | (s[r, :n] == want)).all()
+        assert (s[r, n:] == -np.inf).all() and (w[r, n:] == -1).all() and (b[r, n:] == -1).all()
+    assert m.kernel_error() == 0
+    return s, w, b
+
+
+@pytest.mark.parametrize("R,B,V", FORMS + [(1, 1, 30000), (3, 20, 9000)])
+@pytest.mark.parametrize("score", [-1e9, -1e16, -1e20, -3e38, 1e18, 1e20, 3e38, np.inf])
+def test_scores_beside_which_logits_are_small(p, R, B, V, score):
+    # beams that a program has put far behind (or before) the others: 64 bits do not tell their words' scores apart, their logits do
+    rng = np.random.default_rng(22)
+    x = head(rng, R, B, V)
+    # beams one behind the other, where 64 bits keep some of what a logit adds; else all alike
+    scores = np.full((R, B), score) * (1.0 + np.arange(B) if abs(score) <= 1e18 else 1.0)
+    chosen(p, x, scores, 12)
+    scores[:, 0] = -2.0
+    x[:, 0] = -np.inf
+    x[:, 0, 17:20] = 3.0        # the beam in front has three words
+    chosen(p, x, scores, 40)
+    chosen(p, P.rounded(rng.integers(0, 3, x.shape).astype(np.float64), "F32"), scores, 30)
+
+
+@pytest.mark.parametrize("R,B,V", FORMS)
+@pytest.mark.parametrize("size", [1e-18, 1e-30, 1e-44])
+def test_logits_too_small_to_change_a_score(p, R, B, V, size):
+    rng = np.random.default_rng(23)
+    x = P.rounded(rng.standard_normal((R, B, V)) * size, "F32")
+    chosen(p, x, np.full((R, B), -1.0), 9)
+    x[:, :, 11] = 5.0
+    chosen(p, x, -rng.random((R, B)), 50)
+    chosen(p, x, np.full((R, B), -1.0), 50)
+
+
+def test_ended_beams_among_equal_scores(p):
+    m = b200.load()
+    x = np.zeros((1, 3, 4000), dtype=np.float32)
+    x[0, 2, 3999] = 100.0                     # as good as certain: 64 bits give the score of the ended beam
+    outs = [m.device_array(np.full(4, 77, dtype=np.int32)) for _ in range(3)]
+    keep = [m.device_array(x), m.device_array(np.array([-3.0, -2.0, -2.0], dtype=np.float32)), m.device_array(np.array([0, 1, 0], dtype=np.uint8))]
+    p.BeamSelect(p.F32, 1, 3, 4000, 4, keep[0].ptr, keep[1].ptr, *(o.ptr for o in outs), done=keep[2].ptr, end_token=3000)(None)
+    assert outs[1].download(np.int32, 4).tolist() == [3000, 3999, 0, 1] and outs[2].download(np.int32, 4).tolist() == [1, 2, 0, 0]
