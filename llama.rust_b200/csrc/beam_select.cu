@@ -347,7 +347,8 @@ struct MergeView {
         const double off = offset[b];
         if (off == -INFINITY) return ORDER64_NONE;
         if (m != m) return i == b * per_beam ? order64(off) : ORDER64_NONE;   // an ended beam's only one
-        return order64(value == m ? off : off + ((double)value - (double)m));
+        const double score = value == m ? off : off + ((double)value - (double)m);
+        return score > -INFINITY ? order64(score) : ORDER64_NONE;   // beside a logit of +inf a word has none, and inf - inf is no score
     }
 };
 

@@ -93,6 +93,20 @@ def chosen(p, x, scores, k):
     return s, w, b
 
 
+@pytest.mark.parametrize("R,B,V", FORMS)
+def test_beams_of_infinite_scores(p, R, B, V):
+    # a score of +inf keeps its beam's words in front; beside a logit of +inf no other word is a candidate, whatever the score
+    rng = np.random.default_rng(21)
+    x = head(rng, R, B, V)
+    x[:, 0, ::V // 5] = np.inf
+    x[:, 1] = -np.inf
+    x[:, 1, 77:80] = 1.0
+    scores = -rng.random((R, B))
+    scores[0, :2] = np.inf
+    chosen(p, x, scores, 12)
+    chosen(p, x[:, :2], scores[:, :2], 40)
+
+
 @pytest.mark.parametrize("R,B,V", FORMS + [(1, 1, 30000), (3, 20, 9000)])
 @pytest.mark.parametrize("score", [-1e9, -1e16, -1e20, -3e38, 1e18, 1e20, 3e38, np.inf])
 def test_scores_beside_which_logits_are_small(p, R, B, V, score):
