@@ -24,7 +24,7 @@ constexpr int PX_MAX_PARTS = 64;   // of the shared positions, and of a row's ow
 
 // A warp a row: its parts joined, the sink, the division, the only rounding.  A row that does not come out finite is computed again from what it sees
 // alone: products run over whole tiles, where a position that another row of the block sees meets this one with weight 0, and 0 * Inf is NaN.  So is one whose
-// shared part met a page out of range (maximum NaN, sum 0).  A row whose shared part gave up waiting (both NaN) is not stored.
+// shared part met a page out of range, or scores that F32 holds whole steps of only (maximum NaN, sum 0).  A row whose shared part gave up waiting (both NaN) is not stored.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
     constexpr int C = D / 32, AT_ONCE = 8;   // channels of a lane: C lane ..; parts whose loads are under way together

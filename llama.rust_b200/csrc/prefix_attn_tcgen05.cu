@@ -28,6 +28,9 @@ constexpr int TC_M = 128, TC_N = PX_TILE, TC_THREADS = 384, TC_SM_WARP0 = 4, TC_
 constexpr int TC_REGS = 168, TC_FEW_REGS = 56, TC_MANY_REGS = 216;   // a thread's at launch, then of the loading and of the softmax warps
 constexpr int TC_ERR_WAIT = 4;
 constexpr float TC_MOST = 4096.0f;   // sum of a tile's weights up to which the maximum in use is kept
+// A maximum is rounded, a weight's exponent is not: the largest weight is 2^e with e up to half a step of the maximum.  From this one on that is 1 and more (2^31: weights
+// of the best positions are all zero, or infinite), and the row is computed again position by position
+constexpr float TC_FAR = 16777216.0f;
 static_assert(TC_FEW_REGS * TC_SM_WARP0 * 32 + TC_MANY_REGS * (TC_THREADS - TC_SM_WARP0 * 32) <= TC_REGS * TC_THREADS, "register shares");
 
 template <typename T, int D, int ROWS>
@@ -392,7 +395,7 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
             }
             if (copy == 0 && c0 == 0) {
                 outs[x] = live ? out : -1;
-                if (live) a.ml[out] = !finished ? make_float2(NAN, NAN) : *(volatile int *)&sh.bad ? make_float2(NAN, 0.0f) : make_float2(m, l);
+                if (live) a.ml[out] = !finished ? make_float2(NAN, NAN) : *(volatile int *)&sh.bad || (fabsf(m) >= TC_FAR && m > -INFINITY) ? make_float2(NAN, 0.0f) : make_float2(m, l);
             }
             const int y = TWO ? g * TC_M + r : r;
             if (warp_live) {

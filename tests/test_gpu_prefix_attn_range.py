@@ -1,0 +1,68 @@
+"""b200_prefix_attn where scores are so large that F32 holds whole steps of their logarithm only.  One channel of q and k makes the scores, all of them exact in F32 and far
+apart, so that the best position has all the weight and the result is its value (of two equal best ones the mean).  The bound: its weight may be rounded to the cache's type, half a
+step of it, the result is rounded once more, and F32 sums and quotients are good to 2^-20:  |got - o| <= (half + 2^-20) mean |v| + half |o| + SMALLEST."""
+import numpy as np
+import pytest
+
+import b200
+import plain_paged as P
+from test_gpu_prefix_attn import Problem, one_part, p  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+made = {}   # problems by what shapes them: their values take longer to make than a call
+
+
+def outstanding(p, n, ty, d, factor, value, scale, ats, hints, page=64):
+    """queries with `factor` in channel 0, keys with `value` there at positions `ats`, further below at the others"""
+    if (n, ty, d) not in made:
+        made[n, ty, d] = Problem(p, [n], [900] * n, [896] * n, ty, d, 1, 4, page)
+    pr = made[n, ty, d]
+    pr.p, pr.scale = p, scale
+    pr.q[:] = 0.0
+    pr.q[..., 0] = factor
+    low = 0.5 * value if factor * value * scale > 0 else 2.0 * value
+    pr.k[..., 0] = P.rounded(low * (1.0 + (np.arange(pr.k[..., 0].size).reshape(pr.k[..., 0].shape) % 5) * (-0.0625 if low * factor * scale > 0 else 0.0625)), ty)
+    assert (pr.k[..., 0] * factor * scale <= value * factor * scale - 0.25 * abs(value * factor * scale)).all()
+    cells = []
+    for at in ats:
+        page_id, place = P.cell(pr.tables.tolist(), 0, at, page, pr.n_pages)
+        pr.k[page_id, place, 0, 0] = float(P.rounded(value, ty).item())
+        cells.append(pr.v[page_id, place, 0])
+    pr.call(hints)(None)
+    want, size = sum(cells) / len(cells), sum(map(np.abs, cells)) / len(cells)
+    got = pr.result()
+    assert b200.load().kernel_error() == 0
+    half = P.HALF_STEP[ty]
+    assert (np.abs(got - want) <= (half + 2.0 ** -20) * size + half * np.abs(want) + P.SMALLEST[ty]).all(), (ats, got[0, 0, :4], want[:4])
+
+
+ROWS = [7, 14, 30, 60]   # times four heads: every form of the shared part
+
+
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("value", [1e6, 1.1e7, 1.2e7, 2.9e8, 3.1e9, 1e10, 7.5e10, 1e15, 1e20, 1e30])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_of_bf16(p, n, value, sign):
+    for hints in (True, one_part(n)):
+        for ats in ([5], [400, 640], [895]):
+            outstanding(p, n, "BF16", 128, 1.0, sign * value, 1.0, ats, hints)
+
+
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("value", [300.0, 8848.0, 13264.0, 22880.0, 65504.0])
+@pytest.mark.parametrize("scale", [1.0, -1.0, 0.125, 512.0])
+def test_scores_of_f16(p, n, value, scale):
+    for hints in (True, one_part(n)):
+        for ats in ([5], [400, 640], [895]):
+            for sign in (1.0, -1.0):
+                if value <= 32752.0 or sign * scale > 0:
+                    outstanding(p, n, "F16", 64, 2.0 ** 15, sign * value, scale, ats, hints)
+
+
+def test_best_positions_of_a_row_s_own(p):
+    # far behind them the shared ones
+    for value in (3.1e9, 1e10, 1e20):
+        outstanding(p, 9, "BF16", 64, 1.0, value, 1.0, [3], dict(max_len=900, max_shared=100, max_group=9))
+        outstanding(p, 9, "BF16", 64, 1.0, -value, 1.0, [3], dict(max_len=900, max_shared=100, max_group=9))
