@@ -37,7 +37,8 @@ __global__ void __launch_bounds__(128) prefix_merge_kernel(const PrefixArgs a) {
     const float2 *const ml = a.ml + row * parts;
     pdl_wait();
     const int n = a.lens[s];
-    const float sink = a.sinks ? a.sinks[h] * PX_LOG2E : -INFINITY;
+    float sink = a.sinks ? a.sinks[h] * PX_LOG2E : -INFINITY;
+    if (sink > 3.402823466e38f) sink = 3.402823466e38f;   // the largest sinks: no weight is left beside them
     // the first parts' outputs are asked for before it is known which of them there are
     const float *const acc = a.acc + row * parts * D + C * lane;
     auto load = [&](int i, float (&u)[C]) {

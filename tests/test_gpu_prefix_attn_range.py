@@ -66,3 +66,14 @@ def test_best_positions_of_a_row_s_own(p):
     for value in (3.1e9, 1e10, 1e20):
         outstanding(p, 9, "BF16", 64, 1.0, value, 1.0, [3], dict(max_len=900, max_shared=100, max_group=9))
         outstanding(p, 9, "BF16", 64, 1.0, -value, 1.0, [3], dict(max_len=900, max_shared=100, max_group=9))
+
+
+@pytest.mark.parametrize("n", [2, 30])
+def test_sinks_at_the_ends_of_their_range(p, n):
+    # the largest take all the weight, the lowest none of it
+    most = float(np.finfo(np.float32).max)
+    pr = Problem(p, [n], [300 + i for i in range(n)], [256] * n, "BF16", 64, 1, 4, 16, sinks=True)
+    pr.sinks[:] = [most, 2.5e38, -most, -np.inf]
+    pr.run()
+    got = pr.result()
+    assert not got[:, :2].any() and got[:, 2:].any()
