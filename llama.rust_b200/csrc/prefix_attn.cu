@@ -193,7 +193,7 @@ int prefix_plan(const b200_prefix_attn_args &g, PrefixPlan *p) {
     B200_REQUIRE(g.n_head > 0 && g.n_head <= 65535 && g.n_head % g.cache.n_head_kv == 0, "prefix_attn: %d heads over %lld key heads", g.n_head, (long long)g.cache.n_head_kv);
     B200_REQUIRE(g.n_group >= 0 && g.n_group <= g.n_seq, "prefix_attn: %d groups of %lld sequences", g.n_group, (long long)g.n_seq);
     B200_REQUIRE(g.max_len >= 0 && g.max_shared >= 0 && g.max_group >= 0, "prefix_attn: negative sizes");
-    B200_REQUIRE(fabsf(g.scale) < INFINITY, "prefix_attn: the scale is not finite");
+    B200_REQUIRE(fabsf(g.scale * PX_LOG2E) < INFINITY, "prefix_attn: the scale %g, or log2(e) times it, is not finite", g.scale);
     a.n_seq = (int)g.n_seq;
     a.n_head = g.n_head;
     a.n_group = g.n_group;
