@@ -129,7 +129,7 @@ extern "C" int b200_beam_reorder(const struct b200_beam_reorder_args *args, void
         for (int i = 0; i < 3; i++)
             B200_REQUIRE(!paged_overlap(in[i], in_bytes[i], out[o], out_bytes[o]) && (i >= o || !paged_overlap(out[i], out_bytes[i], out[o], out_bytes[o])), "beam_reorder: an output overlaps another operand");
     for (int i = 0; i < g.n_pools; i++) B200_REQUIRE(g.pools[i] != nullptr && (uintptr_t)g.pools[i] % 16 == 0, "beam_reorder: pool %d is null or not 16-byte aligned", i);
-    const PagedOperand mem[6] = {{g.parents, "parents"}, {g.tables_in, "tables_in"}, {g.tables_out, "tables_out"}, {g.lens_in, "lens_in"}, {g.lens_out, "lens_out"}, {g.row_of, "row_of"}};
+    const PagedOperand mem[6] = {{g.parents, "parents", 4}, {g.tables_in, "tables_in", 4}, {g.tables_out, "tables_out", 4}, {g.lens_in, "lens_in", 4}, {g.lens_out, "lens_out", 4}, {g.row_of, "row_of", 4}};
     int rc = paged_check_device(mem, 6, "beam_reorder");
     for (int i = 0; i < g.n_pools && rc == B200_STATUS_SUCCESS; i++) {
         const PagedOperand pool = {g.pools[i], "a pool"};

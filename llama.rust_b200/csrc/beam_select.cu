@@ -638,7 +638,7 @@ int b200_beam_select(const struct b200_beam_select_args *args, void *stream) {
                          "beam_select: an output or the workspace overlaps another operand");
         for (int i = 0; i < o; i++) B200_REQUIRE(!paged_overlap(out[i], out_bytes[i], out[o], out_bytes[o]), "beam_select: an output or the workspace overlaps another operand");
     }
-    const PagedOperand mem[7] = {{g.logits, "logits"}, {g.scores, "scores"}, {g.done, "done"}, {g.out_scores, "out_scores"}, {g.out_tokens, "out_tokens"}, {g.out_parents, "out_parents"},
+    const PagedOperand mem[7] = {{g.logits, "logits"}, {g.scores, "scores", 4}, {g.done, "done"}, {g.out_scores, "out_scores", 4}, {g.out_tokens, "out_tokens", 4}, {g.out_parents, "out_parents", 4},
                                  {g.workspace, "the workspace"}};
     if ((rc = paged_check_device(mem, 7, "beam_select")) != B200_STATUS_SUCCESS) return rc;
     uint8_t *const ws = (uint8_t *)g.workspace;

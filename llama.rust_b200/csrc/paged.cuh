@@ -19,10 +19,12 @@ struct PagedCache {
 };
 
 int paged_check_cache(const b200_paged_cache &c, const char *op, PagedCache *out);   // paged_append.cu
-// refuses operands (null: not given) that no kernel of the current device may touch: another device's memory, the host's pageable memory
+// refuses operands (null: not given) that are not aligned to their elements, and those that no kernel of the current device may touch: another device's memory, the host's
+// pageable memory
 struct PagedOperand {
     const void *p;
     const char *name;
+    unsigned align = 1;   // bytes of an element, where nothing else has looked at it
 };
 int paged_check_device(const PagedOperand *operands, int n, const char *op);
 inline bool paged_overlap(const void *a, size_t na, const void *b, size_t nb) { return (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na; }

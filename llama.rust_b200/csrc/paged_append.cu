@@ -13,6 +13,7 @@
 namespace b200 {
 
 int paged_check_device(const PagedOperand *operands, int n, const char *op) {
+    for (int i = 0; i < n; i++) B200_REQUIRE((uintptr_t)operands[i].p % operands[i].align == 0, "%s: %s must be aligned to %u bytes", op, operands[i].name, operands[i].align);
     int dev = 0;
     B200_CUDA(cudaGetDevice(&dev));
     for (int i = 0; i < n; i++) {
@@ -199,8 +200,8 @@ extern "C" int b200_paged_append(const struct b200_paged_append_args *args, void
     if (g.n_head) all |= (uintptr_t)g.q;
     const uint64_t out = g.n_head ? (uintptr_t)g.q_out | (uint64_t)nb[6] | (uint64_t)nb[7] : 0;
     B200_REQUIRE(all % xs == 0 && out % 2 == 0, "paged_append: rows and strides must be aligned to their elements");
-    const PagedOperand mem[10] = {{g.cache.k, "the cache's keys"}, {g.cache.v, "the cache's values"}, {g.cache.tables, "tables"}, {g.pos, "pos"}, {g.seq, "seq"},
-                                  {g.k, "k"}, {g.v, "v"}, {g.n_head ? g.q : nullptr, "q"}, {g.n_head ? g.q_out : nullptr, "q_out"}, {g.n_dims ? g.rope : nullptr, "rope"}};
+    const PagedOperand mem[10] = {{g.cache.k, "the cache's keys"}, {g.cache.v, "the cache's values"}, {g.cache.tables, "tables", 4}, {g.pos, "pos", 4}, {g.seq, "seq", 4},
+                                  {g.k, "k"}, {g.v, "v"}, {g.n_head ? g.q : nullptr, "q"}, {g.n_head ? g.q_out : nullptr, "q_out"}, {g.n_dims ? g.rope : nullptr, "rope", 4}};
     if ((rc = paged_check_device(mem, 10, "paged_append")) != B200_STATUS_SUCCESS) return rc;
     a.n_tok = g.n_tok;
     a.pos = g.pos;

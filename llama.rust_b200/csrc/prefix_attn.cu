@@ -260,8 +260,8 @@ int b200_prefix_attn(const struct b200_prefix_attn_args *args, void *stream) {
                  "prefix_attn: q, dst and their strides must be multiples of 16 bytes");
     B200_REQUIRE(g.workspace != nullptr && (uintptr_t)g.workspace % 256 == 0 && g.workspace_nbytes >= p.bytes, "prefix_attn: a workspace of %zu bytes, 256-byte aligned, is needed (%zu given)", p.bytes,
                  g.workspace_nbytes);
-    const PagedOperand mem[10] = {{g.cache.k, "the cache's keys"}, {g.cache.v, "the cache's values"}, {g.cache.tables, "tables"}, {g.q, "q"}, {g.dst, "dst"}, {g.lens, "lens"},
-                                  {g.n_group ? g.shared : nullptr, "shared"}, {g.n_group ? g.group_first : nullptr, "group_first"}, {g.sinks, "sinks"}, {g.workspace, "the workspace"}};
+    const PagedOperand mem[10] = {{g.cache.k, "the cache's keys"}, {g.cache.v, "the cache's values"}, {g.cache.tables, "tables", 4}, {g.q, "q"}, {g.dst, "dst"}, {g.lens, "lens", 4},
+                                  {g.n_group ? g.shared : nullptr, "shared", 4}, {g.n_group ? g.group_first : nullptr, "group_first", 4}, {g.sinks, "sinks", 4}, {g.workspace, "the workspace"}};
     if ((rc = paged_check_device(mem, 10, "prefix_attn")) != B200_STATUS_SUCCESS) return rc;
     PrefixArgs &a = p.a;
     if ((rc = device_error_word(&a.err)) != B200_STATUS_SUCCESS) return rc;
