@@ -90,11 +90,6 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
     static_assert(sizeof(TcShared) <= 256, "barriers");
     TcShared &sh = *(TcShared *)(tc_raw + C::Q + C::SLOTS * C::TILE);
     const uint32_t q_s = pa_smem(tc_raw), kv_s = q_s + C::Q;
-    if (q_s & 1023u) {   // the swizzle counts in 1024 bytes
-        pdl_wait();
-        if (threadIdx.x == 0) atomicExch(a.err, TC_ERR_WAIT);
-        return;
-    }
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     volatile int *abort_flag = &sh.abort_flag;
     int64_t id = blockIdx.x;
@@ -452,12 +447,14 @@ int launch(const PrefixArgs &a, CUtensorMapDataType type, cudaStream_t s) {
                      paged_tile_map(&vm, type, a.cache.v, D, a.cache.n_head_kv, page, a.cache.n_pages, a.cache.page_stride, ta.box),
                  "prefix_attn: tensor maps over %lld pages of %d positions refused", (long long)a.cache.n_pages, page);
     B200_CUDA(cudaFuncSetAttribute(prefix_parts_kernel<T, D, ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
-    // the warps' register shares come out of what the block is launched with
-    static const int regs = [] {
-        cudaFuncAttributes fa;
-        return cudaFuncGetAttributes(&fa, prefix_parts_kernel<T, D, ROWS>) == cudaSuccess ? fa.numRegs : 0;
+    // the warps' register shares come out of what the block is launched with; the swizzle counts in 1024 bytes, where shared memory begins
+    static const cudaFuncAttributes built = [] {
+        cudaFuncAttributes fa = {};
+        if (cudaFuncGetAttributes(&fa, prefix_parts_kernel<T, D, ROWS>) != cudaSuccess) fa.numRegs = 0;
+        return fa;
     }();
-    B200_REQUIRE(regs >= TC_REGS, "prefix_attn: a build with %d registers a thread cannot share them out", regs);
+    B200_REQUIRE(built.numRegs >= TC_REGS && built.sharedSizeBytes == 0, "prefix_attn: a build with %d registers a thread and %zu bytes of static shared memory cannot be served", built.numRegs,
+                 built.sharedSizeBytes);
     const int64_t ctas = (int64_t)a.n_group * a.cache.n_head_kv * a.shared_blocks * a.shared_parts + a.own_ctas;
     return launch_pdl(prefix_parts_kernel<T, D, ROWS>, dim3((unsigned)ctas), dim3(TC_THREADS), C::SMEM, s, km, vm, a, ta);
 }
