@@ -3,7 +3,7 @@
 //
 //   score(b, w) = scores[b] + ((x_w - m) - log sum_v exp(x_v - m)),   m = max_v x_v        (m = +inf: x_w - m is 0 where x_w = m, -inf elsewhere)
 //
-// Bound by reading the logits once, but for the latency of what follows the read.  Two launches, or one of clusters for requests of up to 16 chunks:
+// Bound by reading the logits once, but for the latency of what follows the read.  Two launches, or one of clusters for few requests of up to 16 chunks:
 //   * beam_rows_kernel: a CTA holds a chunk of a row in registers (512 threads x EPT values), so that maximum, sum of exponentials and the chunk's k best come of
 //     one read.  The k best: the k-th largest of the maxima of groups of threads, of which there are 2 k and more, is a bound that at least k values reach and
 //     few more do; those are listed and ordered by counting the better ones of each.  Where more than 512 reach it (equal values), bisections over counts find the k-th value
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(BS_MERGE_NT) beam_merge_kernel(const SelectArg
     beam_merge(a, r, a.cand + slot0 * a.k, a.top + slot0, a.sum + slot0, sh);
 }
 
-// Both in one launch, for requests of up to 16 chunks in all: a cluster a request.  Every CTA leaves its chunk's candidates in the first one's shared memory, which
+// Both in one launch, for few requests of up to 16 chunks in all: a cluster a request.  Every CTA leaves its chunk's candidates in the first one's shared memory, which
 // merges them (4 beams x 32000: 6.0 us of the device, 6.5 in two launches, and 2 us less of the host)
 template <typename T, int EPT>
 __global__ void __launch_bounds__(BS_NT) beam_cluster_kernel(const SelectArgs a) {
@@ -548,10 +548,19 @@ int select_ept(int64_t rows, int64_t n_vocab, int type) {
     return least;
 }
 
-// the same for the form with clusters: the fewest values a thread with which a request has no more chunks than that; 0: none
-int select_cluster_ept(int n_beam, int64_t n_vocab, int type) {
-    for (int ept = type == B200_TYPE_F32 ? 4 : 8; ept <= 16; ept *= 2)
-        if (n_beam * ((n_vocab + BS_NT * ept - 1) / (BS_NT * ept)) <= BS_CLUSTER) return ept;
+// The same for the form with clusters: the fewest values a thread with which a request has no more chunks than that; 0: two launches.  Clusters are quicker while all of
+// them are at work at once, two CTAs an SM (larger ones leave SMs of a group over), and wait for one another beyond; F32, us of the device, clusters and two launches:
+//   CTAs of a request  requests                       requests
+//                   1  296       6.5    8.9             400   11.7   11.6
+//                   2  148       6.5    7.9             160   11.2    8.0
+//                   4   64       6.8    7.5              74    8.6    7.7
+//                   8   18       7.1    7.8              37    9.9    9.0
+//                  16   14       7.5    8.6 (32000 x 4)  16   10.7    9.4 (64: 18.8 and 9.4 at 32000, 114 and 15 at 8 x 5000)
+int select_cluster_ept(int n_request, int n_beam, int64_t n_vocab, int type) {
+    for (int ept = type == B200_TYPE_F32 ? 4 : 8; ept <= 16; ept *= 2) {
+        const int64_t size = n_beam * ((n_vocab + BS_NT * ept - 1) / (BS_NT * ept)), ctas = n_request * size;
+        if (size <= BS_CLUSTER) return 4 * ctas <= (size <= 2 ? 8 : size <= 4 ? 7 : 6) * (int64_t)sm_count() ? ept : 0;
+    }
     return 0;
 }
 
@@ -569,7 +578,7 @@ int select_plan(const b200_beam_select_args &g, SelectPlan *p) {
     B200_REQUIRE(g.k >= 1 && g.k <= BS_MAX_K, "beam_select: %d candidates (1 to %d)", g.k, BS_MAX_K);
     B200_REQUIRE(g.n_vocab >= 1 && g.n_vocab <= (1 << 24) && g.logits_ld >= g.n_vocab, "beam_select: a vocabulary of %lld in rows %lld apart (up to 2^24)", (long long)g.n_vocab, (long long)g.logits_ld);
     p->rows = (int64_t)g.n_request * g.n_beam;
-    p->ept = select_cluster_ept(g.n_beam, g.n_vocab, g.logits_type);
+    p->ept = select_cluster_ept(g.n_request, g.n_beam, g.n_vocab, g.logits_type);
     p->cluster = p->ept > 0;
     if (!p->cluster) p->ept = select_ept(p->rows, g.n_vocab, g.logits_type);
     p->chunks = (g.n_vocab + BS_NT * p->ept - 1) / (BS_NT * p->ept);

@@ -142,3 +142,10 @@ def test_ended_beams_among_equal_scores(p):
     keep = [m.device_array(x), m.device_array(np.array([-3.0, -2.0, -2.0], dtype=np.float32)), m.device_array(np.array([0, 1, 0], dtype=np.uint8))]
     p.BeamSelect(p.F32, 1, 3, 4000, 4, keep[0].ptr, keep[1].ptr, *(o.ptr for o in outs), done=keep[2].ptr, end_token=3000)(None)
     assert outs[1].download(np.int32, 4).tolist() == [3000, 3999, 0, 1] and outs[2].download(np.int32, 4).tolist() == [1, 2, 0, 0]
+
+
+@pytest.mark.parametrize("R,B,V", [(147, 1, 2100), (148, 1, 2100), (149, 1, 2100), (298, 1, 900), (13, 4, 8000), (14, 4, 8000), (15, 4, 8000), (16, 4, 8000), (64, 8, 700)])
+def test_as_many_requests_as_either_form_takes(p, R, B, V):
+    rng = np.random.default_rng(R)
+    select(p, head(rng, R, B, V), -rng.random((R, B)), 2 * B)
+    select(p, head(rng, R, B, V, "BF16"), -rng.random((R, B)), B, "BF16", done=(rng.random((R, B)) < 0.2).astype(int), end=5)
