@@ -64,7 +64,7 @@ int b200_paged_append(const struct b200_paged_append_args *args, void *stream);
  * sequence s the first shared[s] positions are read through the table of its group's first sequence, once for the whole group; the others through its
  * own table.  n_group 0 (group_first and shared null): nothing is shared.  lens[s] <= 0: a row of zeros; a row whose weights are all zero too.
  * Positions that a row does not see may hold anything.  q and dst are of the cache's type; scores, weights' sums and outputs are F32 until the
- * last rounding, weights enter the second product with 16 bits.  max_len, max_shared and max_group (most sequences of a group) shape the launch: larger
+ * last rounding, weights enter the second product with 16 bits.  dst may be q where their strides are the same, else they must not overlap.  max_len, max_shared and max_group (most sequences of a group) shape the launch: larger
  * values on the device are served all the same, only less evenly. */
 struct b200_prefix_attn_args {
     struct b200_paged_cache cache;   /* d 64 or 128 */

@@ -11,10 +11,11 @@
 //   * beam_merge_kernel: a CTA per request joins the chunks' sums in 64 bits and selects among beams x chunks x k candidates the same way, the scores
 //     in 64 bits: two candidates of different beams are told apart unless their scores agree to about 1e-7.
 //   * beam_cluster_kernel: a CTA a chunk leaves its candidates in the first one's shared memory, which merges them.
-// Measured on the device: 64 rows of 128256 F32 (33 MB, 16 candidates) 17 us, 160 of 50001 BF16 15 us, 4 of 32000 F32 6 us.  The chunks' read takes a third of the first; the rest
+// Measured on the device: 64 rows of 128256 F32 (33 MB, 16 candidates) 17.4 us, 160 of 50001 BF16 14.8 us, 4 of 32000 F32 6.1 us.  The chunks' read takes a third of the first; the rest
 // is the latency of barriers and counting, of which an SM overlaps three CTAs.
-// Sums: F32 over a thread's values, 64 bits from there (1e-7 of the sum, so 1e-7 of a score).  The same row gives the same bits wherever it lies:
-// which thread sums which value depends on the vocabulary alone, also where rows do not begin at 16-byte boundaries (their values are then shifted into place).
+// Sums: F32 over a thread's values, 64 bits from there (1e-7 of the sum, so 1e-7 of a score).  Equal rows of one call give the same bits wherever they lie: which thread
+// sums which value is the same for all of them, also where rows do not begin at 16-byte boundaries (their values are then shifted into place).  Calls of other numbers of
+// rows may cut a vocabulary into other chunks, and differ in the last bits of a sum.
 #include <cuda_bf16.h>
 
 #include "paged.cuh"

@@ -14,6 +14,7 @@
 //   * A row sees a tile as a whole or not at all, so that no score is masked one by one.
 //   * A tile's weights are taken under the maximum in use without a look at its scores; only where their sum exceeds 2^12 (or the row has seen nothing yet) are they taken
 //     again under the tile's own maximum, and the output rescaled: the weights' rounding is relative, so nothing is lost.
+//   * Weights enter the second product in the cache's 16 bits, as in the own part (what that costs the outputs stands there).
 // Bound by the chain of a tile: scores of a block in (a product of 128 x 128 x 128 and the way to tensor memory), 128 exponentials a thread, weights back, the second product.  Two blocks take
 // 1.85 us a tile (2 x 8.4 MFLOP and 64 KB: 1.3 PFLOP/s and 5.2 TB/s while 148 SMs are at it), one block 1.25 us.  Under ncu (64 rows behind 32768 positions, two blocks of 128) the tensor cores are busy 28 % of
 // the launch, memory 44 %, issue slots 24 %; the beginning (page ids, queries, first tile) and the end (outputs of 256 rows) are 10 us of 55.  (There 96 CTAs take in 35 GB/s each and 52 of the own part 50: 6 TB/s.)

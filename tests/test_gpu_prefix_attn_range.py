@@ -77,3 +77,20 @@ def test_sinks_at_the_ends_of_their_range(p, n):
     pr.run()
     got = pr.result()
     assert not got[:, :2].any() and got[:, 2:].any()
+
+
+@pytest.mark.parametrize("n", [3, 40])
+def test_outputs_in_the_place_of_the_queries(p, n):
+    # rows that are computed again read their queries after others have been stored
+    pr = Problem(p, [n], [300 + i for i in range(n)], [256] * n, "BF16", 128, 1, 4, 16)
+    page, place = P.cell(pr.tables.tolist(), 0, 77, 16, pr.n_pages)
+    pr.v[page, place, 0, 9] = np.inf
+    pr.q[1, 2, 0] = 2.0 ** 30
+    call = pr.call()
+    call.args.dst = call.args.q
+    call(None)
+    pr.out = pr.keep[3]
+    got = P.values(pr.out.download(np.uint16, pr.q.size), pr.ty).reshape(pr.q.shape)
+    apart = pr.call()
+    apart(None)
+    assert np.array_equal(got, pr.result(), equal_nan=True) and b200.load().kernel_error() == 0
