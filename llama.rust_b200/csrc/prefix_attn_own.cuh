@@ -8,6 +8,9 @@
 namespace b200 {
 
 constexpr int PX_BM = 16, PX_BN = 64, PX_NT = PX_WARPS * 32;
+// F16 has no weights below 2^-24: there a row's maximum counts 15 steps of log2 less, so that its largest weight is 2^15 and one of 2^-29 of it loses nothing
+template <typename T>
+constexpr float PX_LIFT = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 template <int D>
 constexpr int PX_STAGES = D == 128 ? 2 : 4;   // 64 KB of tiles under way or at work
 __device__ __forceinline__ uint32_t px_smem(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -223,7 +226,7 @@ __device__ __forceinline__ void prefix_own_stream(const PrefixArgs &a, int unit,
                 }
             mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 1)); mx_a = fmaxf(mx_a, __shfl_xor_sync(0xffffffffu, mx_a, 2));
             mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 1)); mx_b = fmaxf(mx_b, __shfl_xor_sync(0xffffffffu, mx_b, 2));
-            const float mn_a = fmaxf(m_a, mx_a), mn_b = fmaxf(m_b, mx_b);
+            const float mn_a = fmaxf(m_a, mx_a - PX_LIFT<T>), mn_b = fmaxf(m_b, mx_b - PX_LIFT<T>);
             const float al_a = m_a == -INFINITY ? 0.0f : pa_ex2(m_a - mn_a), al_b = m_b == -INFINITY ? 0.0f : pa_ex2(m_b - mn_b);
             const float sub_a = mn_a == -INFINITY ? 0.0f : mn_a, sub_b = mn_b == -INFINITY ? 0.0f : mn_b;
             const bool same = m_a == mn_a && m_b == mn_b;

@@ -12,7 +12,7 @@
 //     an output of its own; with two blocks each has its block and both read every tile.  While one computes weights the tensor cores have the other's
 //     products.  A thread owns a row; weights go back into tensor memory over the scores they came from, as the A operand of the second product.
 //   * A row sees a tile as a whole or not at all, so that no score is masked one by one.
-//   * A tile's weights are taken under the maximum in use without a look at its scores; only where their sum exceeds 2^12 (or the row has seen nothing yet) are they taken
+//   * A tile's weights are taken under the maximum in use without a look at its scores; only where their sum exceeds TC_MOST (or the row has seen nothing yet) are they taken
 //     again under the tile's own maximum, and the output rescaled: the weights' rounding is relative, so nothing is lost.
 //   * Weights enter the second product in the cache's 16 bits, as in the own part (what that costs the outputs stands there).
 // Bound by the chain of a tile: scores of a block in (a product of 128 x 128 x 128 and the way to tensor memory), 128 exponentials a thread, weights back, the second product.  Two blocks take
@@ -28,7 +28,13 @@ namespace {
 constexpr int TC_M = 128, TC_N = PX_TILE, TC_THREADS = 384, TC_SM_WARP0 = 4, TC_SLOTS_MAX = 8;
 constexpr int TC_REGS = 168, TC_FEW_REGS = 56, TC_MANY_REGS = 216;   // a thread's at launch, then of the loading and of the softmax warps
 constexpr int TC_ERR_WAIT = 4;
-constexpr float TC_MOST = 4096.0f;   // sum of a tile's weights up to which the maximum in use is kept
+// F16 has no weights below 2^-24: there the maximum in use is 8 steps of log2 below the row's, so that a weight loses nothing down to 2^-22 of the largest and is dropped below
+// 2^-33 (without it 2^-14 and 2^-25: behind one outstanding position a tail of 65536 equal ones was lost as a whole)
+template <typename T>
+constexpr float TC_LIFT = std::is_same<T, __half>::value ? 8.0f : 0.0f;
+// sum of a tile's weights up to which the maximum in use is kept: no weight of F16 overflows, and 128 equal ones of a first tile stay below it
+template <typename T>
+constexpr float TC_MOST = std::is_same<T, __half>::value ? 61440.0f : 4096.0f;
 // A maximum is rounded, a weight's exponent is not: the largest weight is 2^e with e up to half a step of the maximum.  From this one on that is 1 and more (2^31: weights
 // of the best positions are all zero, or infinite), and the row is computed again position by position
 constexpr float TC_FAR = 16777216.0f;
@@ -283,7 +289,7 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
 #pragma unroll
                             for (int e = 0; e < 4; e++) mx[e] = fmaxf(mx[e], sign * __uint_as_float(s[c + e]));
                         float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                        top = top == -INFINITY ? -INFINITY : top * fabsf(sc);
+                        top = top == -INFINITY ? -INFINITY : top * fabsf(sc) - TC_LIFT<T>;
                         const float al = sees && top > m ? pa_ex2(m - top) : 1.0f;
                         if (sees) m = fmaxf(m, top);
                         l *= al;
@@ -315,7 +321,7 @@ prefix_parts_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_const
                     }
                     const float2 p0 = pa_split(ps[0]), p1 = pa_split(ps[1]);
                     const float sum = (p0.x + p1.x) + (p0.y + p1.y);
-                    if (anew || !__any_sync(0xffffffffu, sees && !(sum <= TC_MOST))) {
+                    if (anew || !__any_sync(0xffffffffu, sees && !(sum <= TC_MOST<T>))) {
                         if (sees && m > -INFINITY) l += sum;
                         else if (sees && sum != sum) l = sum;   // NaN scores alone
                         break;

@@ -94,3 +94,65 @@ def test_outputs_in_the_place_of_the_queries(p, n):
     apart = pr.call()
     apart(None)
     assert np.array_equal(got, pr.result(), equal_nan=True) and b200.load().kernel_error() == 0
+
+
+def long_tail(p, ty, n, shared, length, peaks, steps, hints, page=256, each=4):
+    """`length` positions of which those in `peaks` outweigh each of the others by 2^steps, the others' values being 1 where the peaks' are 0: channels 0 .. 31 hold the others' share of the
+    weight, channels 32 .. 63 the peaks'.  Pages are named many times over"""
+    m = b200.load()
+    d, heads = 64, each
+    score = float(P.rounded(steps * np.log(2.0), ty).item())
+    k, v = np.zeros((2, page, 1, d)), np.zeros((2, page, 1, d))
+    k[0, peaks, 0, 0] = score
+    v[..., :32] = 1.0
+    v[0, peaks, 0, :32], v[0, peaks, 0, 32:] = 0.0, 1.0
+    q = np.zeros((n, heads, d))
+    q[..., 0] = 1.0
+    tables = np.ones((n, length // page), dtype=np.int32)
+    tables[:, 0] = 0
+    keep = [m.device_array(x) for x in (P.bits(k, ty), P.bits(v, ty), tables, P.bits(q, ty), np.zeros(q.size, dtype=np.uint16), np.full(n, length, dtype=np.int32), np.full(n, shared, dtype=np.int32), np.array([0, n], dtype=np.int32))]
+    cache = p.Cache({"F16": p.F16, "BF16": p.BF16}[ty], page, 2, 1, d, keep[0].ptr, keep[1].ptr, keep[2].ptr, length // page, n)
+    p.PrefixAttn(cache, n, heads, keep[3].ptr, keep[4].ptr, keep[5].ptr, 1.0, shared=keep[6].ptr, group_first=keep[7].ptr, n_group=1, **hints)(None)
+    got = P.values(keep[4].download(np.uint16, q.size), ty).reshape(q.shape)
+    rest = (length - len(peaks)) * np.exp(-score)
+    want = np.repeat([rest / (len(peaks) + rest), len(peaks) / (len(peaks) + rest)], 32)
+    # equal weights: all are rounded alike, by half a step; the result once more; scores and exponentials are good to 2^-20; an output grows in 4096 additions of 16
+    # products, each off by at most 2^-23 of what it has come to: 2^-12 of the whole
+    half = P.HALF_STEP[ty]
+    assert (np.abs(got - want) <= (2 * half + 2.0 ** -19 + 2.0 ** -12) * want + P.SMALLEST[ty]).all(), (got[0, 0, [0, 63]], want[[0, 63]])
+    assert m.kernel_error() == 0
+
+
+@pytest.mark.parametrize("ty", ["F16", "BF16"])
+@pytest.mark.parametrize("steps", [10.0, 15.3, 19.7])
+@pytest.mark.parametrize("n", ROWS)
+def test_many_small_weights_behind_a_shared_position(p, ty, steps, n):
+    long_tail(p, ty, n, 65536, 65536, [0, 128], steps, dict(max_len=1000, max_shared=128, max_group=n))
+
+
+@pytest.mark.parametrize("ty", ["F16", "BF16"])
+@pytest.mark.parametrize("steps", [10.0, 15.3, 19.7, 25.4, 27.8])
+def test_many_small_weights_behind_a_position_of_a_row_s_own(p, ty, steps):
+    long_tail(p, ty, 2, 0, 65536, [0, 16, 32, 48], steps, dict(max_len=64, max_shared=0, max_group=0))
+
+
+@pytest.mark.parametrize("n", ROWS)
+def test_small_weights_of_f16_that_are_rounded_to_whole_steps(p, n):
+    # below 2^-22 of the largest a weight is a multiple of 2^-32 of it: that bounds what a tail may lose, 2^-33 a position
+    m, length = b200.load(), 65536
+    for steps in (23.3, 25.4, 28.6):
+        page, d, heads, score = 256, 64, 4, float(P.rounded(steps * np.log(2.0), "F16").item())
+        k, v = np.zeros((2, page, 1, d)), np.ones((2, page, 1, d))
+        k[0, [0, 128], 0, 0], v[0, [0, 128]] = score, 0.0
+        q = np.zeros((n, heads, d))
+        q[..., 0] = 1.0
+        tables = np.ones((n, length // page), dtype=np.int32)
+        tables[:, 0] = 0
+        keep = [m.device_array(x) for x in (P.bits(k, "F16"), P.bits(v, "F16"), tables, P.bits(q, "F16"), np.zeros(q.size, dtype=np.uint16), np.full(n, length, dtype=np.int32), np.full(n, length, dtype=np.int32), np.array([0, n], dtype=np.int32))]
+        cache = p.Cache(p.F16, page, 2, 1, d, keep[0].ptr, keep[1].ptr, keep[2].ptr, length // page, n)
+        p.PrefixAttn(cache, n, heads, keep[3].ptr, keep[4].ptr, keep[5].ptr, 1.0, shared=keep[6].ptr, group_first=keep[7].ptr, n_group=1, max_len=1000, max_shared=128, max_group=n)(None)
+        got = P.values(keep[4].download(np.uint16, q.size), "F16")
+        rest = (length - 2) * np.exp(-score)
+        want = rest / (2.0 + rest)
+        assert (np.abs(got - want) <= length * 2.0 ** -33 / 2.0 + 2.0 ** -10 * want + P.SMALLEST["F16"]).all(), (steps, got[0], want)
+    assert m.kernel_error() == 0
